@@ -44,6 +44,11 @@ EXPORTED_SYMBOLS = (
     "da_decoding_attn_int8kv_tok",
     "da_decoding_attn_paged_int8kv_tok",
     "da_workspace_bytes_int8kv_tok",
+    "da_kv_cache_append",
+    "da_kv_cache_read",
+    "da_decoding_attn_shared_prefix",
+    "da_decoding_attn_paged_shared_prefix",
+    "da_workspace_bytes_shared_prefix",
     "da_supported_head_dims",
     "da_last_error",
     "da_version",
@@ -143,6 +148,16 @@ def _declare(lib):
     lib.da_decoding_attn_paged_int8kv_tok.argtypes = lib.da_decoding_attn_paged_fp8kv.argtypes
     lib.da_workspace_bytes_int8kv_tok.restype = sz
     lib.da_workspace_bytes_int8kv_tok.argtypes = lib.da_workspace_bytes_fp8kv.argtypes
+    lib.da_kv_cache_append.restype = ci
+    lib.da_kv_cache_append.argtypes = [vp, vp] + [sz] * 4 + [vp] * 5 + [sz] * 10 + [ci] * 3 + [vp] * 3
+    lib.da_kv_cache_read.restype = ci
+    lib.da_kv_cache_read.argtypes = [vp] * 7 + [sz] * 10 + [ci] * 3 + [vp] * 3
+    lib.da_decoding_attn_shared_prefix.restype = ci
+    lib.da_decoding_attn_shared_prefix.argtypes = [vp, vp, vp, sz, vp, vp, vp, vp] + [sz] * 6 + [ci, ci, cf, vp, sz, vp, sz, vp]
+    lib.da_decoding_attn_paged_shared_prefix.restype = ci
+    lib.da_decoding_attn_paged_shared_prefix.argtypes = [vp] * 5 + [sz, vp, vp] + [sz] * 10 + [ci, ci, cf, vp, sz, vp, sz, vp]
+    lib.da_workspace_bytes_shared_prefix.restype = sz
+    lib.da_workspace_bytes_shared_prefix.argtypes = [sz] * 9
     ip = ctypes.POINTER(ci)
     lib.da_plan.restype = ci
     lib.da_plan.argtypes = [sz, sz, sz, sz, sz, sz, ci, sz, ip, ip, ip, ip]

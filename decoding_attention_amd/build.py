@@ -30,6 +30,12 @@ SOURCES = [
     "da_gqa_mfma_i4g.hip",
     "da_gqa_mfma_i8g.hip",
     "da_gqa_mfma_i8t.hip",
+    "da_kv_cache.hip",
+    "da_prefix_d64.hip",
+    "da_prefix_d96.hip",
+    "da_prefix_d128.hip",
+    "da_prefix_d256.hip",
+    "da_prefix_merge.hip",
 ]
 
 # libdecoding_attn_probe.so (measurement aids of bench.py, csrc/decoding_attn_probe.h): the same objects, with

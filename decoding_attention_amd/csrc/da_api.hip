@@ -19,7 +19,9 @@
 #include "decoding_attn_probe.h"
 #endif
 #include "da_gqa_mfma.h"
+#include "da_kv_cache.h"
 #include "da_mla.h"
+#include "da_prefix.h"
 #include "da_sweep_launch.h"
 
 namespace {
@@ -1273,6 +1275,325 @@ int da_decoding_attn(const void* q, const void* k, const void* v, void* o, const
                      void* hip_stream) {
     return da_decoding_attn_ex(q, k, v, o, cu_seq_k, max_seq_k, batch, head_q, head_k, dim, dim_v, is_alibi, is_bf16,
                                0.0f, nullptr, 0, nullptr, 0, hip_stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------------------
+// Rows into a paged cache and back (da_kv_cache.hip)
+
+namespace {
+
+// (const in: the pools of a read are not written)
+int run_kv_cache(bool read, const void* k, const void* v, void* k_out, void* v_out, size_t k_token_stride,
+                 size_t k_head_stride, size_t v_token_stride, size_t v_head_stride, void* k_pages, void* v_pages,
+                 const int32_t* block_table, const int32_t* seq_lens, const int32_t* cu_seq, size_t tokens, size_t batch,
+                 size_t head_k, size_t dim, size_t dim_v, size_t page_size, size_t max_blocks_per_seq, size_t num_pages,
+                 size_t k_page_stride, size_t v_page_stride, int is_bf16, int kv_format, int scale_form, float* k_scale,
+                 float* v_scale, void* hip_stream) {
+    const bool has_v = v_pages != nullptr;
+    if (!k_pages) return fail(DA_ERR_INVALID_ARGUMENT, "k_pages is null");
+    if (read ? (has_v != (v_out != nullptr)) : (has_v != (v != nullptr)))
+        return fail(DA_ERR_INVALID_ARGUMENT, "v and v_pages go together: both or neither");
+    if (!supported_dims(dim, dim_v))
+        return fail(DA_ERR_UNSUPPORTED, "unsupported head dims (dim %zu, dim_v %zu)", dim, dim_v);
+    if (!has_v && dim_v == dim) return fail(DA_ERR_INVALID_ARGUMENT, "v_pages is null (only at (576, 512) V lies inside K)");
+    if (kv_format < DA_KV_FORMAT_16BIT || kv_format > DA_KV_FORMAT_INT4)
+        return fail(DA_ERR_INVALID_ARGUMENT, "kv_format (%d) must be one of DA_KV_FORMAT_*", kv_format);
+    if (scale_form < DA_KV_SCALE_PER_HEAD || scale_form > DA_KV_SCALE_GROUP64)
+        return fail(DA_ERR_INVALID_ARGUMENT, "scale_form (%d) must be one of DA_KV_SCALE_*", scale_form);
+    if (scale_form != DA_KV_SCALE_PER_HEAD) {
+        if (kv_format != DA_KV_FORMAT_INT8 && kv_format != DA_KV_FORMAT_INT4)
+            return fail(DA_ERR_UNSUPPORTED, "(scale, zero) pairs apply to an int8 or int4 cache only");
+        if (dim != dim_v || (dim != 64 && dim != 128 && dim != 256))
+            return fail(DA_ERR_UNSUPPORTED, "(scale, zero) pairs: head dims (64,64), (128,128) and (256,256) only");
+        if (!k_scale || !v_scale) return fail(DA_ERR_INVALID_ARGUMENT, "(scale, zero) pairs: k_scale or v_scale is null");
+        if ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) & 7u)
+            return fail(DA_ERR_INVALID_ARGUMENT, "(scale, zero) pairs must be 8-byte aligned");
+    }
+    if (head_k == 0 || head_k * dim > ((size_t)1 << 18))
+        return fail(DA_ERR_INVALID_ARGUMENT, "head_k (%zu) out of range (1 .. %zu at dim %zu)", head_k, ((size_t)1 << 18) / dim,
+                    dim);
+    Paging pg;
+    const int rc = check_paging(block_table, seq_lens, 0, head_k, dim, dim_v, page_size, max_blocks_per_seq, k_page_stride,
+                                v_page_stride, has_v, &pg);
+    if (rc != DA_OK) return rc;
+    if (!aligned16(k_pages) || (has_v && !aligned16(v_pages)))
+        return fail(DA_ERR_INVALID_ARGUMENT, "k_pages and v_pages must be 16-byte aligned");
+    if (num_pages > (size_t)INT32_MAX || batch > (size_t)INT32_MAX || tokens > (size_t)INT32_MAX)
+        return fail(DA_ERR_INVALID_ARGUMENT, "shape out of range (pages %zu, batch %zu, tokens %zu)", num_pages, batch, tokens);
+    if (!cu_seq && tokens != batch)
+        return fail(DA_ERR_INVALID_ARGUMENT, "without cu_seq there is one token per sequence: tokens (%zu), batch (%zu)", tokens,
+                    batch);
+    if (tokens == 0 || batch == 0) return DA_OK;
+    if (read ? (!k_out || !aligned16(k_out) || !aligned16(v_out)) : (!k || (reinterpret_cast<uintptr_t>(k) & 1u) ||
+                                                                     (reinterpret_cast<uintptr_t>(v) & 1u)))
+        return fail(DA_ERR_INVALID_ARGUMENT, read ? "k and v must be 16-byte aligned, k not null" : "k is null, or k or v misaligned");
+
+    da::KvCacheParams p = {};
+    auto plane = [&](da::KvPlane& pl, const void* src, void* dst, void* pool, float* scale, size_t token_stride,
+                     size_t head_stride, size_t page_stride, size_t d) {
+        pl.src = src;
+        pl.dst = dst;
+        pl.pool = pool;
+        pl.scale = scale;
+        pl.src_token = (int64_t)token_stride;
+        pl.src_head = (int64_t)head_stride;
+        pl.page = (int64_t)page_stride;
+        pl.dim = (int)d;
+        pl.aligned = aligned16(src) && token_stride % 8 == 0 && head_stride % 8 == 0 ? 1 : 0;
+    };
+    plane(p.plane[0], k, k_out, k_pages, k_scale, k_token_stride, k_head_stride, k_page_stride, dim);
+    if (has_v) plane(p.plane[1], v, v_out, v_pages, v_scale, v_token_stride, v_head_stride, v_page_stride, dim_v);
+    p.block_table = block_table;
+    p.seq_lens = seq_lens;
+    p.cu_seq = cu_seq;
+    p.tokens = (int64_t)tokens;
+    p.batch = (int)batch;
+    p.head_k = (int)head_k;
+    while (((size_t)1 << p.page_shift) < page_size) ++p.page_shift;
+    p.max_blocks = (int)max_blocks_per_seq;
+    p.num_pages = (int)num_pages;
+    hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
+    const hipError_t e = (read ? da::launch_kv_read : da::launch_kv_append)(p, is_bf16 != 0, kv_format, scale_form,
+                                                                             has_v ? 2 : 1, stream);
+    if (e != hipSuccess) return fail(DA_ERR_HIP, "cache kernel launch: %s", hipGetErrorString(e));
+    return DA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int da_kv_cache_append(const void* k, const void* v, size_t k_token_stride, size_t k_head_stride, size_t v_token_stride,
+                       size_t v_head_stride, void* k_pages, void* v_pages, const int32_t* block_table,
+                       const int32_t* seq_lens, const int32_t* cu_seq, size_t tokens, size_t batch, size_t head_k,
+                       size_t dim, size_t dim_v, size_t page_size, size_t max_blocks_per_seq, size_t num_pages,
+                       size_t k_page_stride, size_t v_page_stride, int is_bf16, int kv_format, int scale_form,
+                       float* k_scale, float* v_scale, void* hip_stream) {
+    return run_kv_cache(false, k, v, nullptr, nullptr, k_token_stride, k_head_stride, v_token_stride, v_head_stride, k_pages,
+                        v_pages, block_table, seq_lens, cu_seq, tokens, batch, head_k, dim, dim_v, page_size,
+                        max_blocks_per_seq, num_pages, k_page_stride, v_page_stride, is_bf16, kv_format, scale_form, k_scale,
+                        v_scale, hip_stream);
+}
+
+int da_kv_cache_read(const void* k_pages, const void* v_pages, void* k, void* v, const int32_t* block_table,
+                     const int32_t* seq_lens, const int32_t* cu_seq, size_t tokens, size_t batch, size_t head_k, size_t dim,
+                     size_t dim_v, size_t page_size, size_t max_blocks_per_seq, size_t num_pages, size_t k_page_stride,
+                     size_t v_page_stride, int is_bf16, int kv_format, int scale_form, const float* k_scale,
+                     const float* v_scale, void* hip_stream) {
+    return run_kv_cache(true, nullptr, nullptr, k, v, 0, 0, 0, 0, const_cast<void*>(k_pages), const_cast<void*>(v_pages),
+                        block_table, seq_lens, cu_seq, tokens, batch, head_k, dim, dim_v, page_size, max_blocks_per_seq,
+                        num_pages, k_page_stride, v_page_stride, is_bf16, kv_format, scale_form, const_cast<float*>(k_scale),
+                        const_cast<float*>(v_scale), hip_stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------------------
+// Attention behind a shared prefix (da_prefix_kernel.h)
+
+namespace {
+
+struct PrefixPlan {
+    bool wave_per_head = false;
+    int row_tiles = 0, splits = 0, chunk = 0, prefix_wgs = 0;
+    int groups = 0, own_splits = 0, own_chunk = 1, own_groups = 0;
+    long long own_wgs = 0;
+    size_t prefix_parts = 0, own_parts = 0;  // partial rows of either part
+    size_t ws_bytes = 0;
+};
+
+// own_max: most own tokens of a sequence.
+PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t batch, size_t head_q, size_t head_k, size_t dim) {
+    PrefixPlan pl;
+    const long long ratio = (long long)(head_q / head_k), rows = (long long)batch * ratio;
+    const long long tile = dim <= 128 ? 64 : 32;
+    pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
+    long long s = std::max<long long>(1, 256 / ((long long)head_k * pl.row_tiles));
+    s = std::min(s, ((long long)prefix_len + 127) / 128);
+    long long chunk = ((long long)prefix_len + s - 1) / s;
+    chunk = (chunk + tile - 1) / tile * tile;
+    pl.chunk = (int)chunk;
+    pl.splits = (int)(((long long)prefix_len + chunk - 1) / chunk);
+    pl.prefix_wgs = (int)(((long long)head_k * pl.splits + 7) / 8 * 8 * pl.row_tiles);
+    pl.prefix_parts = (size_t)pl.splits * batch * head_q;
+
+    pl.wave_per_head = head_k % 4 == 0;
+    pl.groups = (int)((ratio + 15) / 16);
+    pl.own_groups = (int)(pl.wave_per_head ? head_k / 4 : head_k) * pl.groups;
+    if (own_max > 0) {
+        const long long trip = pl.wave_per_head ? da::kGqaTile : 4 * da::kGqaTile;
+        const long long base = (long long)batch * pl.own_groups;
+        long long ns = std::max<long long>(1, 512 / base);
+        ns = std::max(ns, ((long long)own_max + 1023) / 1024);
+        ns = std::min(ns, ((long long)own_max + trip - 1) / trip);
+        long long oc = ((long long)own_max + ns - 1) / ns;
+        oc = (oc + trip - 1) / trip * trip;
+        pl.own_chunk = (int)oc;
+        pl.own_splits = (int)(((long long)own_max + oc - 1) / oc);
+        const long long segs = (long long)batch * pl.own_splits * (pl.own_groups / pl.groups);
+        pl.own_wgs = pl.groups > 1 ? (segs + 7) / 8 * 8 * pl.groups : segs;
+        pl.own_parts = (size_t)pl.own_splits * batch * head_q;
+    }
+    pl.ws_bytes = (pl.prefix_parts + pl.own_parts) * (dim + 2) * sizeof(float);
+    return pl;
+}
+
+int check_prefix_shape(size_t prefix_len, size_t max_seq_k, size_t batch, size_t head_q, size_t head_k, size_t dim,
+                       size_t dim_v) {
+    if (head_k == 0 || head_q == 0 || head_q % head_k != 0)
+        return fail(DA_ERR_INVALID_ARGUMENT, "head_q (%zu) must be a multiple of head_k (%zu)", head_q, head_k);
+    if (!supported_dims(dim, dim_v) || dim != dim_v)
+        return fail(DA_ERR_UNSUPPORTED, "shared prefix: unsupported head dims (dim %zu, dim_v %zu): supported are (64,64) (96,96) "
+                    "(128,128) (256,256)", dim, dim_v);
+    // (the kernels count query rows, positions and work-groups in 32 bits)
+    if (prefix_len > (size_t)INT32_MAX / 2 || max_seq_k > (size_t)INT32_MAX / 2 || head_q > 65535 || batch > (1u << 24) ||
+        batch * head_q > ((size_t)1 << 28) || ((max_seq_k + 1023) / 1024) * batch * head_q > ((size_t)1 << 28))
+        return fail(DA_ERR_INVALID_ARGUMENT, "shape out of range (prefix_len %zu, max_seq_k %zu, batch %zu, head_q %zu)",
+                    prefix_len, max_seq_k, batch, head_q);
+    return DA_OK;
+}
+
+// table: page ids of the prefix (paged), else null and pk, pv are the prefix's packed rows.
+int run_shared_prefix(const void* q, const void* pk, const void* pv, const int32_t* table, size_t prefix_len, const void* k,
+                      const void* v, void* o, const int32_t* cu_seq_k, const Paging& pg, size_t own_max, size_t batch,
+                      size_t head_q, size_t head_k, size_t dim, int is_alibi, int is_bf16, float softmax_scale,
+                      const float* alibi_slopes, void* workspace, size_t workspace_bytes, void* hip_stream) {
+    if (!q) return fail(DA_ERR_INVALID_ARGUMENT, "q is null");
+    if (!o) return fail(DA_ERR_INVALID_ARGUMENT, "o is null");
+    if (!pk || !pv) return fail(DA_ERR_INVALID_ARGUMENT, "the prefix's K or V is null");
+    if (own_max > 0 && (!k || !v)) return fail(DA_ERR_INVALID_ARGUMENT, "k or v is null");
+    if (!aligned16(q) || !aligned16(pk) || !aligned16(pv) || !aligned16(k) || !aligned16(v) || !aligned16(o))
+        return fail(DA_ERR_INVALID_ARGUMENT, "q, o and all K and V must be 16-byte aligned");
+    if (batch == 0) return DA_OK;
+    const PrefixPlan pl = make_prefix_plan(prefix_len, own_max, batch, head_q, head_k, dim);
+    if (pl.prefix_wgs + pl.own_wgs > (long long)INT32_MAX / 2)
+        return fail(DA_ERR_INVALID_ARGUMENT, "shape out of range (%lld work-groups)", pl.prefix_wgs + pl.own_wgs);
+    hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
+    void* ws = workspace;
+    if (ws) {
+        if (workspace_bytes < pl.ws_bytes)
+            return fail(DA_ERR_WORKSPACE, "workspace has %zu bytes, %zu needed", workspace_bytes, pl.ws_bytes);
+        if (!aligned16(ws)) return fail(DA_ERR_INVALID_ARGUMENT, "workspace must be 16-byte aligned");
+    } else {
+        const int rc = cached_workspace(pl.ws_bytes, stream, &ws);
+        if (rc != DA_OK) return rc;
+    }
+
+    da::PrefixParams p = {};
+    da::SweepParams& w = p.own;
+    float* at = reinterpret_cast<float*>(ws);
+    auto take = [&](size_t floats) {
+        float* const r = at;
+        at += floats;
+        return r;
+    };
+    p.ws_o = take(pl.prefix_parts * dim);
+    w.ws_o = take(pl.own_parts * dim);
+    p.ws_ml = take(pl.prefix_parts * 2);
+    w.ws_ml = take(pl.own_parts * 2);
+    p.k = pk;
+    p.v = pv;
+    p.table = table;
+    p.prefix_len = (int)prefix_len;
+    p.rows = (int)(batch * (head_q / head_k));
+    p.row_tiles = pl.row_tiles;
+    p.splits = pl.splits;
+    p.chunk = pl.chunk;
+    p.prefix_wgs = pl.prefix_wgs;
+    p.own_groups = pl.own_groups;
+    w.q = q;
+    w.k = k;
+    w.v = v;
+    w.o = o;
+    w.cu_seq_k = cu_seq_k;
+    w.slopes = is_alibi ? alibi_slopes : nullptr;
+    w.k_row = w.v_row = (int64_t)(head_k * dim);
+    w.v_head = (int)dim;
+    w.head_q = (int)head_q;
+    w.head_k = (int)head_k;
+    w.ratio = (int)(head_q / head_k);
+    w.groups = pl.groups;
+    w.nsplit = pl.own_splits;
+    w.chunk = pl.own_chunk;
+    w.scale_log2 = (softmax_scale > 0.0f ? softmax_scale : (float)(1.0 / std::sqrt((double)dim))) * da::kLog2e;
+    w.is_alibi = is_alibi ? 1 : 0;
+    w.block_table = pg.table;
+    w.seq_lens = pg.seq_lens;
+    while (pg.table && ((size_t)1 << w.page_shift) < pg.page_size) ++w.page_shift;
+    w.max_blocks = (int)pg.max_blocks;
+    w.k_page = (int64_t)pg.k_page;
+    w.v_page = (int64_t)pg.v_page;
+    w.batch = (int)batch;
+    hipError_t e;
+    const int own_wgs = (int)pl.own_wgs;
+    switch (dim) {
+        case 64: e = da::launch_prefix_d64(p, is_bf16 != 0, pl.wave_per_head, own_wgs, stream); break;
+        case 96: e = da::launch_prefix_d96(p, is_bf16 != 0, pl.wave_per_head, own_wgs, stream); break;
+        case 128: e = da::launch_prefix_d128(p, is_bf16 != 0, pl.wave_per_head, own_wgs, stream); break;
+        default: e = da::launch_prefix_d256(p, is_bf16 != 0, pl.wave_per_head, own_wgs, stream); break;
+    }
+    if (e != hipSuccess) return fail(DA_ERR_HIP, "shared-prefix kernel launch: %s", hipGetErrorString(e));
+    e = da::launch_prefix_merge(p, is_bf16 != 0, (int)dim, stream);
+    if (e != hipSuccess) return fail(DA_ERR_HIP, "merge kernel launch: %s", hipGetErrorString(e));
+    return DA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int da_decoding_attn_shared_prefix(const void* q, const void* k_prefix, const void* v_prefix, size_t prefix_len,
+                                   const void* k, const void* v, void* o, const int32_t* cu_seq_k, size_t max_seq_k,
+                                   size_t batch, size_t head_q, size_t head_k, size_t dim, size_t dim_v, int is_alibi,
+                                   int is_bf16, float softmax_scale, const float* alibi_slopes, size_t total_k,
+                                   void* workspace, size_t workspace_bytes, void* hip_stream) {
+    const int rc = check_prefix_shape(prefix_len, max_seq_k, batch, head_q, head_k, dim, dim_v);
+    if (rc != DA_OK) return rc;
+    if (!cu_seq_k) return fail(DA_ERR_INVALID_ARGUMENT, "cu_seq_k is null");
+    if (prefix_len == 0) {  // (nothing is shared)
+        if (!v) return fail(DA_ERR_INVALID_ARGUMENT, "v is null");
+        return run_attention(q, k, v, o, cu_seq_k, Paging{}, KvFormat{}, max_seq_k, batch, head_q, head_k, dim, dim_v,
+                             is_alibi, is_bf16, softmax_scale, alibi_slopes, total_k, workspace, workspace_bytes, hip_stream);
+    }
+    return run_shared_prefix(q, k_prefix, v_prefix, nullptr, prefix_len, k, v, o, cu_seq_k, Paging{}, max_seq_k, batch, head_q,
+                             head_k, dim, is_alibi, is_bf16, softmax_scale, alibi_slopes, workspace, workspace_bytes,
+                             hip_stream);
+}
+
+int da_decoding_attn_paged_shared_prefix(const void* q, const void* k_pages, const void* v_pages, void* o,
+                                         const int32_t* prefix_blocks, size_t prefix_len, const int32_t* block_table,
+                                         const int32_t* seq_lens, size_t max_seq_k, size_t batch, size_t head_q,
+                                         size_t head_k, size_t dim, size_t dim_v, size_t page_size,
+                                         size_t max_blocks_per_seq, size_t k_page_stride, size_t v_page_stride,
+                                         int is_alibi, int is_bf16, float softmax_scale, const float* alibi_slopes,
+                                         size_t total_k, void* workspace, size_t workspace_bytes, void* hip_stream) {
+    int rc = check_prefix_shape(prefix_len, max_seq_k, batch, head_q, head_k, dim, dim_v);
+    if (rc != DA_OK) return rc;
+    Paging pg;
+    rc = check_paging(block_table, seq_lens, max_seq_k, head_k, dim, dim_v, page_size, max_blocks_per_seq, k_page_stride,
+                      v_page_stride, v_pages != nullptr, &pg);
+    if (rc != DA_OK) return rc;
+    if (!k_pages || !v_pages) return fail(DA_ERR_INVALID_ARGUMENT, "k_pages or v_pages is null");
+    if (prefix_len == 0)
+        return run_attention(q, k_pages, v_pages, o, nullptr, pg, KvFormat{}, max_seq_k, batch, head_q, head_k, dim, dim_v,
+                             is_alibi, is_bf16, softmax_scale, alibi_slopes, total_k, workspace, workspace_bytes, hip_stream);
+    if (!prefix_blocks) return fail(DA_ERR_INVALID_ARGUMENT, "prefix_blocks is null");
+    if (prefix_len % page_size != 0)
+        return fail(DA_ERR_INVALID_ARGUMENT, "prefix_len (%zu) must be a multiple of page_size (%zu): whole pages are shared",
+                    prefix_len, page_size);
+    return run_shared_prefix(q, k_pages, v_pages, prefix_blocks, prefix_len, k_pages, v_pages, o, nullptr, pg,
+                             max_seq_k > prefix_len ? max_seq_k - prefix_len : 0, batch, head_q, head_k, dim, is_alibi, is_bf16,
+                             softmax_scale, alibi_slopes, workspace, workspace_bytes, hip_stream);
+}
+
+size_t da_workspace_bytes_shared_prefix(size_t prefix_len, size_t max_seq_k, size_t batch, size_t head_q, size_t head_k,
+                                        size_t dim, size_t dim_v, size_t total_k, size_t page_size) {
+    if (head_k == 0 || head_q % head_k != 0 || !supported_dims(dim, dim_v) || dim != dim_v || batch == 0) return 0;
+    if (prefix_len == 0) return plan_ws_bytes(max_seq_k, batch, head_q, head_k, dim, dim_v, true, total_k, page_size);
+    const size_t own = page_size == 0 ? max_seq_k : (max_seq_k > prefix_len ? max_seq_k - prefix_len : 0);
+    return make_prefix_plan(prefix_len, own, batch, head_q, head_k, dim).ws_bytes;
 }
 
 }  // extern "C"

@@ -1,0 +1,37 @@
+// Launch interface of the shared-prefix kernels (da_prefix_kernel.h): one query token per sequence over a prefix that
+// all sequences share and each sequence's own tokens behind it.
+#pragma once
+#include "da_common.h"
+
+namespace da {
+
+constexpr int kPrefixRows = 128;  // query rows of a prefix work-group: 32 for each of its four waves
+
+template <int D>
+constexpr int prefix_tile() {  // tokens of a K/V tile in LDS
+    return D <= 128 ? 64 : 32;
+}
+
+struct PrefixParams {
+    SweepParams own;              // the sequences' own tokens; q, o, slopes, scale and head counts serve the prefix too
+    const void* k;                // prefix rows [prefix_len, head_k, dim], or the page pools
+    const void* v;
+    const int32_t* table;         // page ids of the prefix (null: packed rows); pages as own's pools
+    int prefix_len;
+    int rows, row_tiles;          // query rows per KV head (batch * ratio), in tiles of kPrefixRows
+    int splits, chunk;            // prefix splits and tokens per split (a multiple of the tile)
+    int prefix_wgs;               // work-groups in front of own's: 8 * ceil(head_k * splits / 8) * row_tiles
+    int own_groups;               // own's work-groups per sequence and split: (head_k or head_k / 4) * own.groups
+    float* ws_o;                  // [splits, batch * head_q, dim] un-normalised partial outputs
+    float* ws_ml;                 // [splits, batch * head_q, 2] running maximum (log2 units) and denominator
+};
+
+// wave_per_head: own's form with one KV head to a wave (head_k a multiple of 4).  own_wgs: work-groups behind the prefix's.
+hipError_t launch_prefix_d64(const PrefixParams& p, bool is_bf16, bool wave_per_head, int own_wgs, hipStream_t stream);
+hipError_t launch_prefix_d96(const PrefixParams& p, bool is_bf16, bool wave_per_head, int own_wgs, hipStream_t stream);
+hipError_t launch_prefix_d128(const PrefixParams& p, bool is_bf16, bool wave_per_head, int own_wgs, hipStream_t stream);
+hipError_t launch_prefix_d256(const PrefixParams& p, bool is_bf16, bool wave_per_head, int own_wgs, hipStream_t stream);
+// the merge of both parts' partials into o
+hipError_t launch_prefix_merge(const PrefixParams& p, bool is_bf16, int dim, hipStream_t stream);
+
+}  // namespace da

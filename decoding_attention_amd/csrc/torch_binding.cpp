@@ -12,6 +12,7 @@
 #include <torch/extension.h>
 
 #include <optional>
+#include <tuple>
 
 #include "../../include/decoding_attn_hip.h"
 
@@ -316,6 +317,305 @@ at::Tensor dmha_fwd_paged(const at::Tensor &q, const at::Tensor &k_pages, const 
     return o;
 }
 
+// ---- K/V rows into a paged cache and back ----
+
+// What the pools hold and how they are scaled, from the tensors of a cache call.
+struct CacheArgs {
+    int format = DA_KV_FORMAT_16BIT, form = DA_KV_SCALE_PER_HEAD;
+    int64_t pack = 1;  // K/V elements per tensor element
+    int64_t batch = 0, head_k = 0, dim = 0, dim_v = 0, page_size = 0, pages = 0;
+    float *k_scale = nullptr, *v_scale = nullptr;
+    const int32_t *cu_seq = nullptr;
+};
+
+CacheArgs cache_args(const at::Tensor &k_pages, const std::optional<at::Tensor> &v_pages_, const at::Tensor &block_table,
+                     const at::Tensor &seq_lens, const std::optional<at::Tensor> &cu_seq, const int64_t tokens,
+                     const at::ScalarType dtype, const std::optional<at::Tensor> &k_scale,
+                     const std::optional<at::Tensor> &v_scale) {
+    CacheArgs a;
+    TORCH_CHECK(dtype == torch::kFloat16 || dtype == torch::kBFloat16,
+                "Decoding-Attention only support FP16 and BF16 data type");
+    if (k_pages.dtype() == torch::kFloat8_e4m3fn) a.format = DA_KV_FORMAT_FP8;
+    else if (k_pages.dtype() == torch::kInt8) a.format = DA_KV_FORMAT_INT8;
+    else if (k_pages.dtype() == torch::kUInt8) a.format = DA_KV_FORMAT_INT4;
+    else
+        TORCH_CHECK(k_pages.scalar_type() == dtype,
+                    "k_pages must have the rows' dtype (or be float8_e4m3fn, int8, or uint8 holding int4 pairs)");
+    a.pack = a.format == DA_KV_FORMAT_INT4 ? 2 : 1;
+    DA_CHECK_DEVICE(k_pages);
+    DA_CHECK_DEVICE(block_table);
+    DA_CHECK_DEVICE(seq_lens);
+    TORCH_CHECK(block_table.device() == k_pages.device() && seq_lens.device() == k_pages.device(),
+                "k_pages, block_table and seq_lens must share a device");
+    TORCH_CHECK(block_table.dtype() == torch::kInt32, "block_table must have dtype int32");
+    TORCH_CHECK(seq_lens.dtype() == torch::kInt32, "seq_lens must have dtype int32");
+    TORCH_CHECK(k_pages.dim() == 4, "k_pages must have four dimensions (pages, page_size, heads, dim)");
+    TORCH_CHECK(block_table.dim() == 2 && seq_lens.dim() == 1 && block_table.size(0) == seq_lens.size(0),
+                "block_table [batch, max_blocks] and seq_lens [batch] must have one row per sequence");
+    DA_CHECK_CONTIGUOUS(block_table);
+    DA_CHECK_CONTIGUOUS(seq_lens);
+    a.batch = seq_lens.size(0);
+    a.pages = k_pages.size(0);
+    a.page_size = k_pages.size(1);
+    a.head_k = k_pages.size(2);
+    a.dim = k_pages.size(3) * a.pack;
+    auto page_dense = [](const at::Tensor &t) {
+        return t.stride(3) == 1 && t.stride(2) == t.size(3) && t.stride(1) == t.size(2) * t.size(3);
+    };
+    TORCH_CHECK(page_dense(k_pages), "k_pages must be dense within a page");
+    if (v_pages_.has_value()) {
+        const at::Tensor &v = v_pages_.value();
+        TORCH_CHECK(v.dtype() == k_pages.dtype() && v.is_cuda() && v.device() == k_pages.device(),
+                    "v_pages must have k_pages' dtype and device");
+        TORCH_CHECK(v.dim() == 4 && v.size(0) == a.pages && v.size(1) == a.page_size && v.size(2) == a.head_k,
+                    "v_pages must have shape (pages, page_size, head_k, dim_v)");
+        TORCH_CHECK(page_dense(v), "v_pages must be dense within a page");
+        a.dim_v = v.size(3) * a.pack;
+    } else {
+        TORCH_CHECK(a.dim == 576, "without v_pages the values lie inside the K rows: dim 576 only");
+        a.dim_v = 512;
+    }
+    TORCH_CHECK(da_supported_head_dims((size_t)a.dim, (size_t)a.dim_v) == 1, "unsupported head dims (dim ", a.dim,
+                ", dim_v ", a.dim_v, "): supported are (64,64) (96,96) (128,128) (256,256) (576,512)");
+    if (cu_seq.has_value()) {
+        const at::Tensor &c = cu_seq.value();
+        TORCH_CHECK(c.dtype() == torch::kInt32, "cu_seq must have dtype int32");
+        TORCH_CHECK(c.is_cuda() && c.device() == k_pages.device() && c.is_contiguous() && c.dim() == 1 &&
+                        c.size(0) == a.batch + 1,
+                    "cu_seq must be a contiguous GPU tensor of batch + 1 values");
+        a.cu_seq = c.data_ptr<int32_t>();
+    } else {
+        TORCH_CHECK(tokens == a.batch, "without cu_seq there is one token per sequence: tokens ", tokens, ", batch ", a.batch);
+    }
+    // factors per head, or pools of (scale, zero) pairs: one dimension more than k_pages per pair's run
+    const auto form_of = [&](const std::optional<at::Tensor> &t) {
+        return !t.has_value() || t.value().dim() < 4 ? DA_KV_SCALE_PER_HEAD
+                                                     : (t.value().dim() == 4 ? DA_KV_SCALE_PER_TOKEN : DA_KV_SCALE_GROUP64);
+    };
+    a.form = form_of(k_scale);
+    TORCH_CHECK(!v_pages_.has_value() ? !v_scale.has_value() || form_of(v_scale) == a.form : form_of(v_scale) == a.form,
+                "k_scale and v_scale must have the same form");
+    const auto check = [&](const std::optional<at::Tensor> &t, const char *name) -> float * {
+        if (!t.has_value()) return nullptr;
+        const at::Tensor &s = t.value();
+        TORCH_CHECK(a.format != DA_KV_FORMAT_16BIT, name, " applies to a float8_e4m3fn, int8 or int4 K/V cache only");
+        TORCH_CHECK(s.dtype() == torch::kFloat32 && s.is_cuda() && s.device() == k_pages.device() && s.is_contiguous(), name,
+                    " must be a contiguous float32 GPU tensor");
+        if (a.form == DA_KV_SCALE_PER_HEAD) {
+            TORCH_CHECK(s.numel() == a.head_k, name, " must hold head_k values");
+        } else {
+            TORCH_CHECK(a.format == DA_KV_FORMAT_INT8 || a.format == DA_KV_FORMAT_INT4,
+                        "(scale, zero) pairs apply to an int8 or int4 K/V cache only");
+            TORCH_CHECK(s.size(0) == a.pages && s.size(1) == a.page_size && s.size(2) == a.head_k && s.size(-1) == 2 &&
+                            (a.form == DA_KV_SCALE_PER_TOKEN || (s.dim() == 5 && s.size(3) * 64 == a.dim)),
+                        name, " must have shape (pages, page_size, head_k, 2) or (pages, page_size, head_k, dim / 64, 2)");
+        }
+        return s.data_ptr<float>();
+    };
+    a.k_scale = check(k_scale, "k_scale");
+    a.v_scale = check(v_scale, "v_scale");
+    return a;
+}
+
+void kv_append(const at::Tensor &k, const std::optional<at::Tensor> &v_, const at::Tensor &k_pages,
+               const std::optional<at::Tensor> &v_pages_, const at::Tensor &block_table, const at::Tensor &seq_lens,
+               const std::optional<at::Tensor> &cu_seq, const std::optional<at::Tensor> &k_scale,
+               const std::optional<at::Tensor> &v_scale) {
+    TORCH_CHECK(k.dim() == 3, "k must have three dimensions (tokens, heads, dim)");
+    const CacheArgs a =
+        cache_args(k_pages, v_pages_, block_table, seq_lens, cu_seq, k.size(0), k.scalar_type(), k_scale, v_scale);
+    TORCH_CHECK(v_.has_value() == v_pages_.has_value(), "v and v_pages go together: both or neither");
+    const auto check = [&](const at::Tensor &t, const char *name, int64_t d) {
+        TORCH_CHECK(t.is_cuda() && t.device() == k_pages.device() && t.dtype() == k.dtype(), name,
+                    " must be on k_pages' device and have k's dtype");
+        TORCH_CHECK(t.dim() == 3 && t.size(0) == k.size(0) && t.size(1) == a.head_k && t.size(2) == d, name,
+                    " must have shape (tokens, head_k, dim)");
+        TORCH_CHECK(t.stride(2) == 1, name, " must have contiguous last dimension");
+    };
+    check(k, "k", a.dim);
+    if (v_.has_value()) check(v_.value(), "v", a.dim_v);
+    if (k.size(0) == 0) return;  // (an empty tensor has no address to pass on)
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k.device());
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(k.device().index()).stream();
+    const at::Tensor *v = v_.has_value() ? &v_.value() : nullptr;
+    const int rc = da_kv_cache_append(
+        k.data_ptr(), v ? v->data_ptr() : nullptr, (size_t)k.stride(0), (size_t)k.stride(1), v ? (size_t)v->stride(0) : 0,
+        v ? (size_t)v->stride(1) : 0, k_pages.data_ptr(), v ? v_pages_.value().data_ptr() : nullptr,
+        block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), a.cu_seq, (size_t)k.size(0), (size_t)a.batch,
+        (size_t)a.head_k, (size_t)a.dim, (size_t)a.dim_v, (size_t)a.page_size, (size_t)block_table.size(1), (size_t)a.pages,
+        (size_t)(k_pages.stride(0) * a.pack), v ? (size_t)(v_pages_.value().stride(0) * a.pack) : 0,
+        k.dtype() == torch::kBFloat16 ? 1 : 0, a.format, a.form, a.k_scale, a.v_scale, (void *)stream);
+    TORCH_CHECK(rc == DA_OK, "kv_cache_append failed (", rc, "): ", da_last_error());
+}
+
+std::tuple<at::Tensor, std::optional<at::Tensor>> kv_read(
+    const at::Tensor &k_pages, const std::optional<at::Tensor> &v_pages_, const at::Tensor &block_table,
+    const at::Tensor &seq_lens, const std::optional<at::Tensor> &cu_seq, const int64_t tokens, const bool is_bf16,
+    const std::optional<at::Tensor> &k_scale, const std::optional<at::Tensor> &v_scale,
+    const std::optional<at::Tensor> &k_out, const std::optional<at::Tensor> &v_out) {
+    const at::ScalarType dtype = is_bf16 ? torch::kBFloat16 : torch::kFloat16;
+    TORCH_CHECK(tokens >= 0, "tokens must not be negative");
+    const CacheArgs a = cache_args(k_pages, v_pages_, block_table, seq_lens, cu_seq, tokens, dtype, k_scale, v_scale);
+    TORCH_CHECK(v_pages_.has_value() || !v_out.has_value(), "v and v_pages go together: both or neither");
+    const auto rows = [&](const std::optional<at::Tensor> &t, const char *name, int64_t d) {
+        if (!t.has_value()) return torch::empty({tokens, a.head_k, d}, k_pages.options().dtype(dtype));
+        const at::Tensor &o = t.value();
+        TORCH_CHECK(o.is_cuda() && o.device() == k_pages.device() && o.scalar_type() == dtype && o.is_contiguous() &&
+                        o.dim() == 3 && o.size(0) == tokens && o.size(1) == a.head_k && o.size(2) == d,
+                    name, " must be a contiguous (tokens, head_k, dim) tensor of the asked dtype on k_pages' device");
+        return o;
+    };
+    at::Tensor k = rows(k_out, "k", a.dim);
+    std::optional<at::Tensor> v;
+    if (v_pages_.has_value()) v = rows(v_out, "v", a.dim_v);
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(k_pages.device());
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(k_pages.device().index()).stream();
+    const int rc = tokens == 0 ? DA_OK : da_kv_cache_read(
+        k_pages.data_ptr(), v ? v_pages_.value().data_ptr() : nullptr, k.data_ptr(), v ? v->data_ptr() : nullptr,
+        block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), a.cu_seq, (size_t)tokens, (size_t)a.batch,
+        (size_t)a.head_k, (size_t)a.dim, (size_t)a.dim_v, (size_t)a.page_size, (size_t)block_table.size(1), (size_t)a.pages,
+        (size_t)(k_pages.stride(0) * a.pack), v ? (size_t)(v_pages_.value().stride(0) * a.pack) : 0, is_bf16 ? 1 : 0,
+        a.format, a.form, a.k_scale, a.v_scale, (void *)stream);
+    TORCH_CHECK(rc == DA_OK, "kv_cache_read failed (", rc, "): ", da_last_error());
+    return {k, v};
+}
+
+// ---- attention behind a shared prefix ----
+
+// Checks that both layouts share, the output, the slopes, and the workspace from torch's stream-aware allocator.
+struct PrefixArgs {
+    int64_t batch = 0, head_q = 0, dim = 0;
+    at::Tensor o, ws;
+    const float *slopes = nullptr;
+    float scale = 0.0f;
+};
+
+PrefixArgs prefix_args(const at::Tensor &q, const std::optional<at::Tensor> &o_, const int64_t dim_v,
+                       const std::optional<double> softmax_scale, const std::optional<at::Tensor> &alibi_slopes) {
+    PrefixArgs a;
+    TORCH_CHECK(q.dtype() == torch::kFloat16 || q.dtype() == torch::kBFloat16,
+                "Decoding-Attention only support FP16 and BF16 data type");
+    DA_CHECK_DEVICE(q);
+    TORCH_CHECK(q.dim() == 3, "q must have three dimensions (batch, heads, dim)");
+    DA_CHECK_CONTIGUOUS(q);
+    a.batch = q.size(0);
+    a.head_q = q.size(1);
+    a.dim = q.size(2);
+    TORCH_CHECK(a.batch > 0, "batch size must be positive");
+    TORCH_CHECK(a.dim == dim_v && da_supported_head_dims((size_t)a.dim, (size_t)dim_v) == 1, "unsupported head dims (dim ",
+                a.dim, ", dim_v ", dim_v, ") behind a shared prefix: supported are (64,64) (96,96) (128,128) (256,256)");
+    if (o_.has_value()) {
+        a.o = o_.value();
+        TORCH_CHECK(a.o.dtype() == q.dtype(), "Output must have the same dtype as inputs");
+        DA_CHECK_DEVICE(a.o);
+        TORCH_CHECK(a.o.device() == q.device(), "o must be on q's device");
+        DA_CHECK_SHAPE(a.o, a.batch, a.head_q, dim_v);
+        DA_CHECK_CONTIGUOUS(a.o);
+    } else {
+        a.o = torch::empty({a.batch, a.head_q, dim_v}, q.options());
+    }
+    if (alibi_slopes.has_value()) {
+        const at::Tensor &s = alibi_slopes.value();
+        TORCH_CHECK(s.dtype() == torch::kFloat32 && s.is_cuda() && s.device() == q.device() && s.is_contiguous() &&
+                        s.numel() == a.head_q,
+                    "alibi_slopes must be a contiguous float32 GPU tensor of head_q values");
+        a.slopes = s.data_ptr<float>();
+    }
+    a.scale = softmax_scale.has_value() ? (float)softmax_scale.value() : 0.0f;
+    return a;
+}
+
+void prefix_workspace(PrefixArgs &a, const at::Tensor &q, size_t prefix_len, size_t max_seq_k, size_t head_k, size_t total_k,
+                      size_t page_size) {
+    const size_t bytes = da_workspace_bytes_shared_prefix(prefix_len, max_seq_k, (size_t)a.batch, (size_t)a.head_q, head_k,
+                                                          (size_t)a.dim, (size_t)a.dim, total_k, page_size);
+    if (bytes > 0) a.ws = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kUInt8));
+}
+
+at::Tensor dmha_fwd_prefix(const at::Tensor &q, const at::Tensor &k_prefix, const at::Tensor &v_prefix, const at::Tensor &k,
+                           const at::Tensor &v, const std::optional<at::Tensor> &o_, const at::Tensor &cu_seq_k,
+                           const int64_t max_seq_k, const int64_t dim_v, const bool is_alibi,
+                           const std::optional<double> softmax_scale, const std::optional<at::Tensor> &alibi_slopes) {
+    PrefixArgs a = prefix_args(q, o_, dim_v, softmax_scale, alibi_slopes);
+    TORCH_CHECK(max_seq_k >= 0, "max_seq_k must not be negative");
+    TORCH_CHECK(cu_seq_k.dtype() == torch::kInt32, "cu_seq_k must have dtype int32");
+    DA_CHECK_DEVICE(cu_seq_k);
+    DA_CHECK_CONTIGUOUS(cu_seq_k);
+    DA_CHECK_SHAPE(cu_seq_k, a.batch + 1);
+    TORCH_CHECK(cu_seq_k.device() == q.device(), "q and cu_seq_k must share a device");
+    TORCH_CHECK(k_prefix.dim() == 3 && k.dim() == 3, "k and k_prefix must have three dimensions (tokens, heads, dim)");
+    const int64_t head_k = k_prefix.size(1);
+    TORCH_CHECK(head_k > 0 && a.head_q % head_k == 0, "number of heads in key/value must divide number of heads in query");
+    const auto check = [&](const at::Tensor &t, const at::Tensor &like, const char *name) {
+        TORCH_CHECK(t.dtype() == q.dtype() && t.is_cuda() && t.device() == q.device(), name,
+                    " must have q's dtype and device");
+        TORCH_CHECK(t.dim() == 3 && t.size(0) == like.size(0) && t.size(1) == head_k && t.size(2) == a.dim, name,
+                    " must have shape (tokens, head_k, dim)");
+        TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+    };
+    check(k_prefix, k_prefix, "k_prefix");
+    check(v_prefix, k_prefix, "v_prefix");
+    check(k, k, "k");
+    check(v, k, "v");
+    const size_t prefix_len = (size_t)k_prefix.size(0), total_k = (size_t)k.size(0);
+    // (no row at all: no sequence has tokens of its own, whatever the bound says)
+    const size_t own_max = total_k == 0 ? 0 : (size_t)max_seq_k;
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index()).stream();
+    if (prefix_len == 0 && total_k == 0) return a.o.zero_();
+    prefix_workspace(a, q, prefix_len, own_max, (size_t)head_k, total_k, 0);
+    const int rc = da_decoding_attn_shared_prefix(
+        q.data_ptr(), k_prefix.data_ptr(), v_prefix.data_ptr(), prefix_len, k.data_ptr(), v.data_ptr(), a.o.data_ptr(),
+        cu_seq_k.data_ptr<int32_t>(), own_max, (size_t)a.batch, (size_t)a.head_q, (size_t)head_k, (size_t)a.dim,
+        (size_t)dim_v, is_alibi ? 1 : 0, q.dtype() == torch::kBFloat16 ? 1 : 0, a.scale, a.slopes, total_k,
+        a.ws.defined() ? a.ws.data_ptr() : nullptr, a.ws.defined() ? (size_t)a.ws.numel() : 0, (void *)stream);
+    TORCH_CHECK(rc == DA_OK, "decoding_attn (shared prefix) failed (", rc, "): ", da_last_error());
+    return a.o;
+}
+
+at::Tensor dmha_fwd_paged_prefix(const at::Tensor &q, const at::Tensor &k_pages, const at::Tensor &v_pages,
+                                 const std::optional<at::Tensor> &o_, const at::Tensor &prefix_blocks,
+                                 const int64_t prefix_len, const at::Tensor &block_table, const at::Tensor &seq_lens,
+                                 const int64_t max_seq_k, const int64_t dim_v, const bool is_alibi,
+                                 const std::optional<double> softmax_scale,
+                                 const std::optional<at::Tensor> &alibi_slopes, const int64_t total_k) {
+    PrefixArgs a = prefix_args(q, o_, dim_v, softmax_scale, alibi_slopes);
+    TORCH_CHECK(max_seq_k >= 0 && prefix_len >= 0, "max_seq_k and prefix_len must not be negative");
+    TORCH_CHECK(k_pages.dim() == 4, "k_pages must have four dimensions (pages, page_size, heads, dim)");
+    const int64_t page_size = k_pages.size(1), head_k = k_pages.size(2);
+    TORCH_CHECK(head_k > 0 && a.head_q % head_k == 0, "number of heads in key/value must divide number of heads in query");
+    for (const at::Tensor *t : {&k_pages, &v_pages}) {
+        TORCH_CHECK(t->dtype() == q.dtype() && t->is_cuda() && t->device() == q.device(),
+                    "k_pages and v_pages must have q's dtype and device");
+        TORCH_CHECK(t->sizes() == k_pages.sizes() && t->size(3) == a.dim,
+                    "k_pages and v_pages must have shape (pages, page_size, head_k, dim)");
+        TORCH_CHECK(t->stride(3) == 1 && t->stride(2) == t->size(3) && t->stride(1) == t->size(2) * t->size(3),
+                    "k_pages and v_pages must be dense within a page");
+    }
+    for (const at::Tensor *t : {&prefix_blocks, &block_table, &seq_lens}) {
+        TORCH_CHECK(t->dtype() == torch::kInt32, "prefix_blocks, block_table and seq_lens must have dtype int32");
+        TORCH_CHECK(t->is_cuda() && t->device() == q.device() && t->is_contiguous(),
+                    "prefix_blocks, block_table and seq_lens must be contiguous and on q's device");
+    }
+    TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == a.batch, "block_table must have one row per sequence");
+    DA_CHECK_SHAPE(seq_lens, a.batch);
+    TORCH_CHECK(prefix_blocks.dim() == 1 && page_size > 0 && prefix_blocks.size(0) * page_size >= prefix_len,
+                "prefix_blocks must hold prefix_len / page_size page ids");
+    c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+    hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index()).stream();
+    const size_t hint = total_k > 0 ? (size_t)total_k : 0;
+    prefix_workspace(a, q, (size_t)prefix_len, (size_t)max_seq_k, (size_t)head_k, hint, (size_t)page_size);
+    const int rc = da_decoding_attn_paged_shared_prefix(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), a.o.data_ptr(), prefix_blocks.data_ptr<int32_t>(),
+        (size_t)prefix_len, block_table.data_ptr<int32_t>(), seq_lens.data_ptr<int32_t>(), (size_t)max_seq_k,
+        (size_t)a.batch, (size_t)a.head_q, (size_t)head_k, (size_t)a.dim, (size_t)dim_v, (size_t)page_size,
+        (size_t)block_table.size(1), (size_t)k_pages.stride(0), (size_t)v_pages.stride(0), is_alibi ? 1 : 0,
+        q.dtype() == torch::kBFloat16 ? 1 : 0, a.scale, a.slopes, hint, a.ws.defined() ? a.ws.data_ptr() : nullptr,
+        a.ws.defined() ? (size_t)a.ws.numel() : 0, (void *)stream);
+    TORCH_CHECK(rc == DA_OK, "decoding_attn (paged, shared prefix) failed (", rc, "): ", da_last_error());
+    return a.o;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -331,4 +631,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
           pybind11::arg("softmax_scale") = pybind11::none(), pybind11::arg("alibi_slopes") = pybind11::none(),
           pybind11::arg("total_k") = 0, pybind11::arg("k_scale") = pybind11::none(),
           pybind11::arg("v_scale") = pybind11::none());
+    m.def("kv_append", &kv_append, "K/V rows into a paged cache", pybind11::arg("k"), pybind11::arg("v_"),
+          pybind11::arg("k_pages"), pybind11::arg("v_pages_"), pybind11::arg("block_table"), pybind11::arg("seq_lens"),
+          pybind11::arg("cu_seq"), pybind11::arg("k_scale"), pybind11::arg("v_scale"));
+    m.def("kv_read", &kv_read, "K/V rows out of a paged cache", pybind11::arg("k_pages"), pybind11::arg("v_pages_"),
+          pybind11::arg("block_table"), pybind11::arg("seq_lens"), pybind11::arg("cu_seq"), pybind11::arg("tokens"),
+          pybind11::arg("is_bf16"), pybind11::arg("k_scale"), pybind11::arg("v_scale"), pybind11::arg("k_out"),
+          pybind11::arg("v_out"));
+    m.def("fwd_prefix", &dmha_fwd_prefix, "Forward pass behind a shared prefix", pybind11::arg("q"),
+          pybind11::arg("k_prefix"), pybind11::arg("v_prefix"), pybind11::arg("k"), pybind11::arg("v"),
+          pybind11::arg("o_"), pybind11::arg("cu_seq_k"), pybind11::arg("max_seq_k"), pybind11::arg("dim_v"),
+          pybind11::arg("is_alibi"), pybind11::arg("softmax_scale"), pybind11::arg("alibi_slopes"));
+    m.def("fwd_paged_prefix", &dmha_fwd_paged_prefix, "Forward pass behind a shared prefix, paged K/V",
+          pybind11::arg("q"), pybind11::arg("k_pages"), pybind11::arg("v_pages"), pybind11::arg("o_"),
+          pybind11::arg("prefix_blocks"), pybind11::arg("prefix_len"), pybind11::arg("block_table"),
+          pybind11::arg("seq_lens"), pybind11::arg("max_seq_k"), pybind11::arg("dim_v"), pybind11::arg("is_alibi"),
+          pybind11::arg("softmax_scale"), pybind11::arg("alibi_slopes"), pybind11::arg("total_k"));
 }

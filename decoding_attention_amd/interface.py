@@ -182,3 +182,106 @@ def decoding_attn_paged_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: Opt
     return _extension().fwd_paged(q, k_pages, v_pages, out, block_table, seq_lens, int(max_seq_k), int(dim_v),
                                   bool(is_alibi), None if softmax_scale is None else float(softmax_scale),
                                   alibi_slopes, int(total_k), k_scale, v_scale)
+
+
+def decoding_attn_shared_prefix_fwd(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor,
+                                    v: torch.Tensor, cu_seq_k: torch.Tensor, max_seq_k: int, dim_v: int, is_alibi: bool,
+                                    *, softmax_scale: Optional[float] = None,
+                                    alibi_slopes: Optional[torch.Tensor] = None,
+                                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """
+    The same attention for a batch whose sequences begin with the same tokens: the prefix's K and V are read once for the
+    whole batch instead of once per sequence (no counterpart in the reference).
+
+    Arguments:
+        q: [batch, head_q, dim], torch.float16 / torch.bfloat16; one query token per sequence.
+        k_prefix, v_prefix: [prefix_len, head_k, dim], same dtype; the keys of every sequence begin with these.
+        k, v: [total_k, head_k, dim], same dtype; each sequence's own tokens behind the prefix.
+        cu_seq_k: [batch + 1], torch.int32 cumulative numbers of own tokens; a sequence may have none.
+        max_seq_k: maximum number of own tokens in the batch.
+        dim_v: head dimension of v, equal to dim: 64, 96, 128 or 256.
+        is_alibi: whether to add the ALiBi bias slope_h * (j - (len - 1)), len counting the prefix.
+        softmax_scale, alibi_slopes (keyword only): as for decoding_attn_fwd.
+    Return:
+        o: [batch, head_q, dim_v], same dtype as q.
+    """
+    q, k_prefix, v_prefix, k, v = [maybe_contiguous(x) for x in (q, k_prefix, v_prefix, k, v)]
+    return _extension().fwd_prefix(q, k_prefix, v_prefix, k, v, out, cu_seq_k, int(max_seq_k), int(dim_v), bool(is_alibi),
+                                   None if softmax_scale is None else float(softmax_scale), alibi_slopes)
+
+
+def decoding_attn_paged_shared_prefix_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                                          prefix_blocks: torch.Tensor, prefix_len: int, block_table: torch.Tensor,
+                                          seq_lens: torch.Tensor, max_seq_k: int, dim_v: int, is_alibi: bool, *,
+                                          softmax_scale: Optional[float] = None,
+                                          alibi_slopes: Optional[torch.Tensor] = None, total_k: int = 0,
+                                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """
+    The same over a paged K/V cache: the arguments of decoding_attn_paged_fwd, whole sequences, plus the pages they share.
+
+    Arguments:
+        prefix_blocks: torch.int32 page ids of the shared prefix in token order (the first entries of every sequence's
+            block table row; the row's own first entries are not read).
+        prefix_len: tokens of the prefix, a multiple of the page size; 0 is decoding_attn_paged_fwd itself.
+        seq_lens: [batch], torch.int32 key tokens of each sequence, prefix included.  A sequence shorter than the prefix
+            (a padded row of the batch, length 0) gets a zero output row.
+        The others as for decoding_attn_paged_fwd and decoding_attn_shared_prefix_fwd; 16-bit pools.
+    Return:
+        o: [batch, head_q, dim_v], same dtype as q.
+    """
+    q = maybe_contiguous(q)
+    return _extension().fwd_paged_prefix(q, k_pages, v_pages, out, prefix_blocks, int(prefix_len), block_table, seq_lens,
+                                         int(max_seq_k), int(dim_v), bool(is_alibi),
+                                         None if softmax_scale is None else float(softmax_scale), alibi_slopes,
+                                         int(total_k))
+
+
+def kv_cache_append(k: torch.Tensor, v: Optional[torch.Tensor], k_pages: torch.Tensor, v_pages: Optional[torch.Tensor],
+                    block_table: torch.Tensor, seq_lens: torch.Tensor, cu_seq: Optional[torch.Tensor] = None, *,
+                    k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+    """
+    Write the new K/V rows of every sequence into a paged cache, quantised on the way (no counterpart in the reference).
+
+    Arguments:
+        k, v: [tokens, head_k, dim] and [tokens, head_k, dim_v], torch.float16 / torch.bfloat16, any strides with a dense
+            last dimension (columns of a fused projection's output).  v is None when V lies inside K (576).
+        k_pages, v_pages, block_table: the cache as decoding_attn_paged_fwd takes it, in any of its formats.
+        seq_lens: [batch], torch.int32 key tokens of each sequence AFTER the call; the call's tokens are the last ones.
+        cu_seq: [batch + 1], torch.int32 cumulative numbers of the call's tokens; None: one token per sequence.  Rows of
+            k and v behind cu_seq[batch] are skipped, and so is a token that has no place in the cache (a sequence of
+            length 0, a page id outside the pools).
+        k_scale, v_scale (keyword only): as for decoding_attn_paged_fwd.  float32 [head_k] factors are read (default 1);
+            pools of (scale, zero) pairs, [pages, page_size, head_k, 2] or [pages, page_size, head_k, dim / 64, 2], are
+            written beside the rows, with the scheme of quantize_int4_per_token and its kin (the pair in float32, the
+            quotients in float64).
+    A page that is written must belong to one sequence.
+    """
+    if k.stride(-1) != 1:
+        k = k.contiguous()
+    if v is not None and v.stride(-1) != 1:
+        v = v.contiguous()
+    _extension().kv_append(k, v, k_pages, v_pages, block_table, seq_lens, cu_seq, k_scale, v_scale)
+
+
+def kv_cache_read(k_pages: torch.Tensor, v_pages: Optional[torch.Tensor], block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, cu_seq: Optional[torch.Tensor], tokens: int, *, dtype: torch.dtype,
+                  k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                  k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None):
+    """
+    Gather the last rows of every sequence out of a paged cache, de-quantised to 16 bits: the counterpart of
+    kv_cache_append, and with cu_seq the cumulative seq_lens the whole cache in the packed layout of decoding_attn_fwd.
+
+    Arguments:
+        k_pages, v_pages, block_table, seq_lens, k_scale, v_scale: the cache, as for decoding_attn_paged_fwd.
+        cu_seq: [batch + 1], torch.int32 cumulative numbers of rows to read; None: the last row of each sequence.
+        tokens: rows of the result (a host integer: nothing here synchronises).  Rows behind cu_seq[batch] are left as
+            they were; a row that has no place in the cache reads as zeros.
+        dtype (keyword only): torch.float16 / torch.bfloat16; a 16-bit cache's own type.
+        k_out, v_out (keyword only): results to fill, allocated when absent.
+    Return:
+        k [tokens, head_k, dim], v [tokens, head_k, dim_v] (None without v_pages).
+    """
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("Decoding-Attention only support FP16 and BF16 data type")
+    return _extension().kv_read(k_pages, v_pages, block_table, seq_lens, cu_seq, int(tokens), dtype == torch.bfloat16,
+                                k_scale, v_scale, k_out, v_out)

@@ -304,6 +304,83 @@ size_t da_workspace_bytes_int8kv_tok(size_t max_seq_k, size_t batch, size_t head
                                      size_t dim_v, size_t total_k, size_t page_size);
 
 /*
+ * K/V rows written into the page pools of a cache, quantised on the way, and read back (no counterpart in the reference,
+ * whose callers fill their caches themselves).  Block table, lengths, page sizes and strides are those of
+ * da_decoding_attn_paged, so the tensors of the attention call serve here too.
+ *
+ *   cu_seq       device, int32 [batch + 1] prefix offsets of the call's tokens, or NULL: one token per sequence (a decode
+ *                step; tokens == batch).  The tokens of sequence b are the LAST ones of its seq_lens[b]: append is called
+ *                with the lengths that the cache has afterwards, which the attention call behind it takes as well.
+ *   tokens       rows of k and v.  Rows behind cu_seq[batch] are neither read nor written.
+ *   k, v         append: 16-bit rows (is_bf16) [tokens, head_k, dim], dense within a head, token_stride and head_stride
+ *                elements apart (columns of a fused projection's output can be passed as they lie); 16-byte aligned rows
+ *                load 16 bytes at a time, others element by element.  read: dense, 16-byte aligned.
+ *                NULL v and v_pages at (576, 512): V lies inside the K rows.
+ *   num_pages    pages of the pools.  A token whose position is negative (a padded sequence of length 0) or behind the
+ *                block table, or whose page id is not below num_pages, is not written, and reads as zeros.
+ *   kv_format    DA_KV_FORMAT_*: 16-bit (copied), FP8 e4m3, int8, int4 (layouts of the attention entry points)
+ *   scale_form   DA_KV_SCALE_PER_HEAD: k_scale, v_scale are float [head_k] factors s > 0, or NULL for 1; append stores x / s
+ *                rounded to the format (nearest, ties to even), saturating (FP8: at +-448).
+ *                DA_KV_SCALE_PER_TOKEN, DA_KV_SCALE_GROUP64 (int8 and int4; head dims 64, 128, 256): k_scale, v_scale are the
+ *                pools of float (scale, zero) pairs, [pages, page_size, head_k, 2] or [pages, page_size, head_k, dim / 64, 2],
+ *                dense; append WRITES the pairs of its rows: scale = (max - min) / (2^bits - 1), at least 1e-8, zero =
+ *                qmin - min / scale, and n = x / scale + zero rounded to the nearest integer (ties to even), clamped.
+ * A page that append writes must belong to one sequence: two tokens that lie in one row of the pools race.  NaN: stored as
+ * NaN in FP8, as 0 in int8 and int4 with factors per head; with pairs it makes the pair, and so the whole row (or run), NaN.
+ */
+#define DA_KV_FORMAT_16BIT 0
+#define DA_KV_FORMAT_FP8 1
+#define DA_KV_FORMAT_INT8 2
+#define DA_KV_FORMAT_INT4 3
+#define DA_KV_SCALE_PER_HEAD 0
+#define DA_KV_SCALE_PER_TOKEN 1
+#define DA_KV_SCALE_GROUP64 2
+int da_kv_cache_append(const void *k, const void *v, size_t k_token_stride, size_t k_head_stride, size_t v_token_stride,
+                       size_t v_head_stride, void *k_pages, void *v_pages, const int32_t *block_table,
+                       const int32_t *seq_lens, const int32_t *cu_seq, size_t tokens, size_t batch, size_t head_k,
+                       size_t dim, size_t dim_v, size_t page_size, size_t max_blocks_per_seq, size_t num_pages,
+                       size_t k_page_stride, size_t v_page_stride, int is_bf16, int kv_format, int scale_form,
+                       float *k_scale, float *v_scale, void *hip_stream);
+
+int da_kv_cache_read(const void *k_pages, const void *v_pages, void *k, void *v, const int32_t *block_table,
+                     const int32_t *seq_lens, const int32_t *cu_seq, size_t tokens, size_t batch, size_t head_k,
+                     size_t dim, size_t dim_v, size_t page_size, size_t max_blocks_per_seq, size_t num_pages,
+                     size_t k_page_stride, size_t v_page_stride, int is_bf16, int kv_format, int scale_form,
+                     const float *k_scale, const float *v_scale, void *hip_stream);
+
+/*
+ * Attention for a batch that shares a prefix: sequence b's keys are the prefix_len prefix tokens followed by its own.  The
+ * prefix's K and V are read once for the whole batch, on the matrix cores, instead of once per sequence (no counterpart in
+ * the reference).  Head dims (64,64), (96,96), (128,128) and (256,256), 16-bit K/V, any head grouping, ALiBi over the whole
+ * sequence (the query token is the last one).
+ *
+ *   packed  k_prefix, v_prefix [prefix_len, head_k, dim]; k, v, cu_seq_k, max_seq_k, total_k describe the own tokens as
+ *           da_decoding_attn_ex's do (max_seq_k 0 and NULL k, v: no sequence has any).  A sequence without own tokens
+ *           attends the prefix alone.
+ *   paged   block_table, seq_lens and max_seq_k describe whole sequences, prefix included, as da_decoding_attn_paged's do;
+ *           the prefix (a whole number of pages) is read through prefix_blocks (int32, prefix_len / page_size page ids), and
+ *           the first prefix_len / page_size entries of the block table's rows are not read.  A sequence shorter than the
+ *           prefix (a padded row of the batch, length 0) gets zero output rows.
+ * prefix_len == 0 is the call without a prefix.  Workspace from da_workspace_bytes_shared_prefix (page_size 0 = packed).
+ */
+int da_decoding_attn_shared_prefix(const void *q, const void *k_prefix, const void *v_prefix, size_t prefix_len,
+                                   const void *k, const void *v, void *o, const int32_t *cu_seq_k, size_t max_seq_k,
+                                   size_t batch, size_t head_q, size_t head_k, size_t dim, size_t dim_v, int is_alibi,
+                                   int is_bf16, float softmax_scale, const float *alibi_slopes, size_t total_k,
+                                   void *workspace, size_t workspace_bytes, void *hip_stream);
+
+int da_decoding_attn_paged_shared_prefix(const void *q, const void *k_pages, const void *v_pages, void *o,
+                                         const int32_t *prefix_blocks, size_t prefix_len, const int32_t *block_table,
+                                         const int32_t *seq_lens, size_t max_seq_k, size_t batch, size_t head_q,
+                                         size_t head_k, size_t dim, size_t dim_v, size_t page_size,
+                                         size_t max_blocks_per_seq, size_t k_page_stride, size_t v_page_stride,
+                                         int is_alibi, int is_bf16, float softmax_scale, const float *alibi_slopes,
+                                         size_t total_k, void *workspace, size_t workspace_bytes, void *hip_stream);
+
+size_t da_workspace_bytes_shared_prefix(size_t prefix_len, size_t max_seq_k, size_t batch, size_t head_q, size_t head_k,
+                                        size_t dim, size_t dim_v, size_t total_k, size_t page_size);
+
+/*
  * Launch plan the library would use for this shape, for tests and benchmarks:
  *   kernel_kind 1 = VALU sweep, 2 = latent (MLA) MFMA sweep, 3 = grouped-head MFMA sweep (also the latent form with
  *   16 query heads or fewer); nsplit = sequence splits;

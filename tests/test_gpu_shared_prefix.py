@@ -1,0 +1,340 @@
+"""Attention behind a shared prefix (decoding_attn_shared_prefix_fwd and its paged form) against a float64 softmax.
+
+Tolerance, for a row with weights w over N tokens (u = half a step of the type): every probability is rounded to 16 bits on
+its way into the second product and the denominator sums the rounded ones, so that the output moves by at most
+u sum w |v - o|; the result is rounded once, u |o|; both products, the sums and the exponential are float32: N 2^-24
+sum w |v| for the sums over the tokens, and 2^-20 (1 + max |x|) of the same for scores x, their scale and exp2.  fp16: a
+probability below 2^-14 of the largest has an absolute error, at most 2^-25 each; results below 2^-14 likewise.
+"""
+import math
+
+import pytest
+import torch
+
+from decoding_attention_amd import (decoding_attn_fwd, decoding_attn_paged_fwd, decoding_attn_paged_shared_prefix_fwd,
+                                    decoding_attn_shared_prefix_fwd, kv_cache_append, kv_cache_read)
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def reference(q, kp, vp, ks, vs, is_alibi, scale=None, slopes=None, live=None):
+    """(o, tolerance) in float64: q [batch, heads, dim]; kp, vp the prefix; ks, vs a list of every sequence's own rows."""
+    batch, hq, d = q.shape
+    hk = kp.shape[1]
+    ratio = hq // hk
+    u = torch.finfo(q.dtype).eps / 2
+    scale = 1 / math.sqrt(d) if scale is None else scale
+    o, tol = torch.zeros(batch, hq, d, dtype=torch.float64), torch.zeros(batch, hq, d, dtype=torch.float64)
+    for b in range(batch):
+        if live is not None and not live[b]:
+            continue
+        k = torch.cat([kp, ks[b]]).double().repeat_interleave(ratio, dim=1)
+        v = torch.cat([vp, vs[b]]).double().repeat_interleave(ratio, dim=1)
+        n = k.shape[0]
+        if n == 0:
+            continue
+        x = torch.bmm(k.permute(1, 0, 2).contiguous(), q[b].double()[:, :, None])[..., 0] * scale  # [heads, n]
+        if is_alibi:
+            s = slopes.double() if slopes is not None else 2.0 ** (-8.0 * torch.arange(1, hq + 1, dtype=torch.float64) / hq)
+            x = x + s[:, None] * (torch.arange(n, dtype=torch.float64) - (n - 1))
+        w = torch.softmax(x, dim=-1)
+        vt = v.permute(1, 0, 2).contiguous()
+        o[b] = torch.bmm(w[:, None, :], vt)[:, 0]
+        spread = torch.bmm(w[:, None, :], (vt - o[b][:, None, :]).abs())[:, 0]
+        size = torch.bmm(w[:, None, :], vt.abs())[:, 0]
+        top = x.abs().amax(dim=-1, keepdim=True)
+        tol[b] = 1.01 * u * (spread + o[b].abs()) + (n * 2.0 ** -24 + 2.0 ** -20 * (1 + top)) * size
+        if q.dtype == torch.float16:
+            tol[b] += n * 2.0 ** -25 * vt.abs().amax() + 2.0 ** -25
+    return o, tol
+
+
+def make(batch, hq, hk, d, prefix, own, dtype, seed=0, sharp=1.0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype)  # noqa: E731
+    q = (torch.randn(batch, hq, d, generator=g) * sharp).to(dtype)
+    kp, vp = r(prefix, hk, d), r(prefix, hk, d)
+    ks, vs = [r(n, hk, d) for n in own], [r(n, hk, d) for n in own]
+    return q, kp, vp, ks, vs
+
+
+def packed(ks, vs, hk, d, dtype):
+    cu = torch.tensor([0] + [k.shape[0] for k in ks]).cumsum(0).to(torch.int32)
+    return torch.cat(ks).to(DEV), torch.cat(vs).to(DEV), cu.to(DEV), max(k.shape[0] for k in ks)
+
+
+def paged(kp, vp, ks, vs, page, seed=0, padded=()):
+    """Pools with shuffled pages, NaN wherever no token lies; the rows' own entries of the prefix are no pages at all."""
+    g = torch.Generator().manual_seed(seed)
+    pre = kp.shape[0] // page
+    assert pre * page == kp.shape[0]
+    blocks = [(k.shape[0] + page - 1) // page for k in ks]
+    n = pre + sum(blocks) + 2
+    order = torch.randperm(n, generator=g).tolist()
+    pk = torch.full((n, page) + kp.shape[1:], float("nan"), dtype=kp.dtype)
+    pv = pk.clone()
+    ids = [order.pop() for _ in range(pre)]
+    for i, p in enumerate(ids):
+        pk[p], pv[p] = kp[i * page:(i + 1) * page], vp[i * page:(i + 1) * page]
+    table = torch.full((len(ks), pre + max(1, max(blocks))), -1, dtype=torch.int32)
+    lens = []
+    for b, k in enumerate(ks):
+        for i in range(blocks[b]):
+            p = order.pop()
+            table[b, pre + i] = p
+            rows = k[i * page:(i + 1) * page]
+            pk[p, :rows.shape[0]], pv[p, :rows.shape[0]] = rows, vs[b][i * page:(i + 1) * page]
+        lens.append(0 if b in padded else kp.shape[0] + k.shape[0])
+    return (pk.to(DEV), pv.to(DEV), torch.tensor(ids, dtype=torch.int32, device=DEV), table.to(DEV),
+            torch.tensor(lens, dtype=torch.int32, device=DEV), max(lens))
+
+
+def check(got, ref):
+    o, tol = ref
+    got = got.cpu().double()
+    assert torch.isfinite(got).all()
+    over = ((got - o).abs() - tol).max().item()
+    assert over <= 0, f"{over:.3e} over the tolerance; largest error {(got - o).abs().max().item():.3e}"
+
+
+OWN = [0, 1, 5, 33, 64, 200, 31, 2]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("hq,hk", [(8, 8), (16, 4), (6, 2), (20, 1), (7, 7), (33, 1), (15, 5)])
+def test_head_layouts(hq, hk, d, dtype):
+    q, kp, vp, ks, vs = make(8, hq, hk, d, 133, OWN, dtype, seed=d + hq)
+    k, v, cu, most = packed(ks, vs, hk, d, dtype)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
+
+
+@pytest.mark.parametrize("prefix", [1, 2, 31, 32, 33, 63, 64, 65, 127, 128, 129, 1000, 4097])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_prefix_lengths(prefix, d):
+    dtype = torch.bfloat16 if prefix % 2 else torch.float16
+    q, kp, vp, ks, vs = make(3, 8, 4, d, prefix, [0, 7, 130], dtype, seed=prefix)
+    k, v, cu, most = packed(ks, vs, 4, d, dtype)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
+
+
+@pytest.mark.parametrize("batch", [1, 2, 31, 32, 33, 65, 130])
+@pytest.mark.parametrize("d", [64, 128])
+def test_batch_sizes(batch, d):
+    """Row tiles that end inside a wave, a work-group, and several of them."""
+    own = [(b * 37) % 50 for b in range(batch)]
+    q, kp, vp, ks, vs = make(batch, 8, 2, d, 300, own, torch.bfloat16, seed=batch)
+    k, v, cu, most = packed(ks, vs, 2, d, torch.bfloat16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
+
+
+@pytest.mark.parametrize("custom", [False, True])
+@pytest.mark.parametrize("d,hq,hk", [(64, 8, 8), (128, 16, 4), (256, 20, 1), (96, 12, 3)])
+def test_alibi_and_scale(d, hq, hk, custom):
+    q, kp, vp, ks, vs = make(8, hq, hk, d, 517, OWN, torch.float16, seed=d)
+    k, v, cu, most = packed(ks, vs, hk, d, torch.float16)
+    scale, slopes = (0.031, torch.rand(hq) * 0.1) if custom else (None, None)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, True, softmax_scale=scale,
+                                        alibi_slopes=None if slopes is None else slopes.to(DEV))
+    check(o, reference(q, kp, vp, ks, vs, True, scale, slopes))
+
+
+@pytest.mark.parametrize("page", [1, 2, 8, 16, 32, 64, 256])
+@pytest.mark.parametrize("d,hq,hk,alibi", [(128, 16, 4, False), (64, 6, 2, True), (96, 8, 8, False), (256, 33, 1, True)])
+def test_pages(d, hq, hk, alibi, page):
+    """Own tokens that end inside pages, rows of the batch without a sequence, poisoned unused rows."""
+    prefix = 256 if page == 256 else 192
+    q, kp, vp, ks, vs = make(8, hq, hk, d, prefix, OWN, torch.bfloat16, seed=page + d)
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=page, padded=(2, 7))
+    o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, lens, most, d, alibi)
+    check(o, reference(q, kp, vp, ks, vs, alibi, live=[b not in (2, 7) for b in range(8)]))
+    assert (o[2] == 0).all() and (o[7] == 0).all()
+
+
+def test_sequences_shorter_than_the_prefix_get_zero_rows():
+    q, kp, vp, ks, vs = make(4, 8, 4, 128, 64, [10, 0, 3, 0], torch.float16)
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, 16)
+    lens[3] = 63
+    o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, 64, table, lens, most, 128, False)
+    check(o, reference(q, kp, vp, ks, vs, False, live=[True, True, True, False]))
+
+
+def test_combined_pool_views():
+    q, kp, vp, ks, vs = make(4, 8, 4, 128, 64, [10, 40, 3, 0], torch.float16)
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, 16)
+    pool = torch.stack([pk, pv], dim=1).contiguous()
+    o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pool[:, 0], pool[:, 1], ids, 64, table, lens, most, 128, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
+
+
+def test_no_prefix_and_no_own_tokens():
+    q, kp, vp, ks, vs = make(4, 8, 4, 128, 100, [0, 0, 0, 0], torch.bfloat16)
+    k, v, cu, most = packed(ks, vs, 4, 128, torch.bfloat16)
+    args = q.to(DEV), kp.to(DEV), vp.to(DEV)
+    check(decoding_attn_shared_prefix_fwd(*args, k, v, cu, most, 128, False), reference(q, kp, vp, ks, vs, False))
+    # (a bound that no sequence reaches)
+    check(decoding_attn_shared_prefix_fwd(*args, k, v, cu, 500, 128, False), reference(q, kp, vp, ks, vs, False))
+    none = kp[:0].to(DEV)
+    assert (decoding_attn_shared_prefix_fwd(q.to(DEV), none, none, k, v, cu, most, 128, False) == 0).all()
+    q, kp, vp, ks, vs = make(4, 8, 4, 128, 0, [3, 0, 70, 9], torch.bfloat16)
+    k, v, cu, most = packed(ks, vs, 4, 128, torch.bfloat16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), none, none, k, v, cu, most, 128, False)
+    assert torch.equal(o, decoding_attn_fwd(q.to(DEV), k, v, cu, most, 128, False))
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, 16)
+    o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, 0, table, lens, most, 128, False)
+    assert torch.equal(o, decoding_attn_paged_fwd(q.to(DEV), pk, pv, table, lens, most, 128, False))
+
+
+@pytest.mark.parametrize("sharp", [0.0, 8.0, 60.0])
+def test_flat_and_steep_scores(sharp):
+    """Equal weights, and one token that takes all the weight, in the prefix or behind it."""
+    q, kp, vp, ks, vs = make(8, 8, 2, 128, 700, OWN, torch.bfloat16, seed=4, sharp=sharp)
+    k, v, cu, most = packed(ks, vs, 2, 128, torch.bfloat16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 128, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
+
+
+def test_a_maximum_that_rises_all_the_way():
+    """Keys in the order of their scores: the running maximum is raised again and again."""
+    q, kp, vp, ks, vs = make(4, 4, 1, 64, 2000, [3, 300, 0, 9], torch.float16, seed=5, sharp=0.1)
+    ramp = torch.linspace(-60, 60, 2000)
+    q[:, :, 0], kp[:, 0, 0] = 8.0, ramp.half()
+    k, v, cu, most = packed(ks, vs, 1, 64, torch.float16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 64, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
+
+
+def test_non_finite_values_stay_with_their_sequences():
+    """A NaN among one sequence's own tokens reaches that sequence alone; one in the prefix reaches all."""
+    q, kp, vp, ks, vs = make(6, 8, 4, 128, 128, [4, 50, 0, 9, 33, 1], torch.bfloat16, seed=6)
+    vs[1][7, 2, 5] = float("nan")
+    ks[4][0, 0, 0] = float("inf")
+    k, v, cu, most = packed(ks, vs, 4, 128, torch.bfloat16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 128, False).cpu()
+    assert torch.isnan(o[1, 4:6, 5]).all() and torch.isfinite(o[[0, 2, 3, 5]]).all()
+    kp[100, 1] = float("nan")
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 128, False).cpu()
+    assert torch.isnan(o[:, 2:4]).all() and torch.isfinite(o[[0, 2, 3, 5]][:, :2]).all()
+
+
+def test_long_prefix_and_large_batch():
+    """Many splits, several row tiles, a prefix beyond one split of each; spot checks."""
+    own = [(b * 53) % 700 for b in range(200)]
+    q, kp, vp, ks, vs = make(200, 32, 8, 128, 9001, own, torch.bfloat16, seed=7)
+    k, v, cu, most = packed(ks, vs, 8, 128, torch.bfloat16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 128, False)
+    rows = [0, 31, 32, 63, 64, 99, 128, 199]
+    check(o[rows], reference(q[rows], kp, vp, [ks[b] for b in rows], [vs[b] for b in rows], False))
+
+
+def test_same_bits_twice_and_on_another_stream():
+    q, kp, vp, ks, vs = make(8, 16, 4, 128, 900, OWN, torch.bfloat16, seed=8)
+    k, v, cu, most = packed(ks, vs, 4, 128, torch.bfloat16)
+    args = (q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 128, False)
+    a = decoding_attn_shared_prefix_fwd(*args)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        b = decoding_attn_shared_prefix_fwd(*args)
+    c = decoding_attn_shared_prefix_fwd(*args)  # (both streams at once)
+    torch.cuda.synchronize()
+    assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_replays_from_a_graph_with_other_lengths():
+    """Two captured graphs of one call, replayed with eager work between; the lengths live on the device."""
+    q, kp, vp, ks, vs = make(8, 16, 4, 128, 256, OWN, torch.bfloat16, seed=9)
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, 16)
+    dq = q.to(DEV)
+
+    def run():
+        return decoding_attn_paged_shared_prefix_fwd(dq, pk, pv, ids, 256, table, lens, most, 128, False)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    g = torch.Generator().manual_seed(10)
+    full = lens.clone()
+    for step in range(4):
+        dq.copy_(torch.randn(q.shape, generator=g).to(q.dtype))
+        lens.copy_(torch.where(torch.arange(8, device=DEV) == step, torch.zeros_like(full), full - (full > 256).int() * step % 2))
+        for graph, out in graphs:
+            graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out, want)
+        assert (want[step] == 0).all()
+
+
+def test_entry_point_with_its_own_and_the_callers_workspace():
+    from decoding_attention_amd import _lib
+    lib = _lib.load()
+    q, kp, vp, ks, vs = make(8, 16, 4, 128, 300, OWN, torch.float16, seed=11)
+    k, v, cu, most = packed(ks, vs, 4, 128, torch.float16)
+    dq, dkp, dvp = q.to(DEV), kp.to(DEV), vp.to(DEV)
+    need = lib.da_workspace_bytes_shared_prefix(300, most, 8, 16, 4, 128, 128, k.shape[0], 0)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)  # (NaN everywhere)
+    outs = []
+    for ptr, size in ((ws.data_ptr(), need), (None, 0)):
+        o = torch.full((8, 16, 128), float("nan"), dtype=torch.float16, device=DEV)
+        call = lambda b: lib.da_decoding_attn_shared_prefix(  # noqa: E731
+            dq.data_ptr(), dkp.data_ptr(), dvp.data_ptr(), 300, k.data_ptr(), v.data_ptr(), o.data_ptr(), cu.data_ptr(), most,
+            8, 16, 4, 128, 128, 0, 0, 0.0, None, k.shape[0], ptr, b, torch.cuda.current_stream().cuda_stream)
+        assert call(size) == 0, _lib.last_error()
+        torch.cuda.synchronize()
+        outs.append(o)
+        if ptr:
+            assert call(size - 16) == _lib.DA_ERR_WORKSPACE
+    check(outs[0], reference(q, kp, vp, ks, vs, False))
+    assert torch.equal(outs[0], outs[1])
+    assert lib.da_release_workspaces() == 0
+
+
+def test_a_serving_loop():
+    """The operators together: a prefix and prompts appended to a paged cache, decode steps that append a row per sequence and
+    attend behind the prefix, and the cache read back at the end.  Every step against float64, and against the attention that
+    reads the whole block table."""
+    hk, hq, d, page, prefix, dtype = 4, 16, 128, 16, 160, torch.bfloat16
+    prompts = [17, 1, 40, 0, 64]
+    steps, batch = 4, 5
+    own = [n + steps for n in prompts]
+    q, kp, vp, ks, vs = make(batch, hq, hk, d, prefix, own, dtype, seed=12)
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=13)
+    pk.fill_(0), pv.fill_(0)
+    # the prefix is written once, through the first sequence's pages
+    table[:, :prefix // page] = ids
+    kv_cache_append(kp.to(DEV), vp.to(DEV), pk, pv, table[:1].contiguous(), torch.tensor([prefix], dtype=torch.int32, device=DEV),
+                    torch.tensor([0, prefix], dtype=torch.int32, device=DEV))
+    cu = torch.tensor([0] + prompts).cumsum(0).to(torch.int32).to(DEV)
+    now = torch.tensor([prefix + n for n in prompts], dtype=torch.int32, device=DEV)
+    kv_cache_append(torch.cat([k[:n] for k, n in zip(ks, prompts)]).to(DEV), torch.cat([v[:n] for v, n in zip(vs, prompts)]).to(DEV),
+                    pk, pv, table, now, cu)
+    g = torch.Generator().manual_seed(14)
+    for step in range(steps):
+        now += 1
+        kv_cache_append(torch.stack([k[n + step] for k, n in zip(ks, prompts)]).to(DEV),
+                        torch.stack([v[n + step] for v, n in zip(vs, prompts)]).to(DEV), pk, pv, table, now)
+        q = torch.randn(batch, hq, d, generator=g).to(dtype)
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, now, most, d, False)
+        seen_k, seen_v = ([t[:n + step + 1] for t, n in zip(x, prompts)] for x in (ks, vs))
+        ref = reference(q, kp, vp, seen_k, seen_v, False)
+        check(o, ref)
+        check(decoding_attn_paged_fwd(q.to(DEV), pk, pv, table, now, most, d, False), ref)
+    assert torch.equal(now, lens)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int32, device=DEV), lens.cumsum(0).to(torch.int32)])
+    k, v = kv_cache_read(pk, pv, table, lens, cu, int(cu[-1]), dtype=dtype)
+    assert torch.equal(k.cpu(), torch.cat([torch.cat([kp, t]) for t in ks]))
+    assert torch.equal(v.cpu(), torch.cat([torch.cat([vp, t]) for t in vs]))
