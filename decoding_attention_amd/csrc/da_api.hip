@@ -1408,7 +1408,7 @@ struct PrefixPlan {
 PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t batch, size_t head_q, size_t head_k, size_t dim) {
     PrefixPlan pl;
     const long long ratio = (long long)(head_q / head_k), rows = (long long)batch * ratio;
-    const long long tile = dim <= 128 ? 64 : 32;
+    const long long tile = 32;
     pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
     long long s = std::max<long long>(1, 256 / ((long long)head_k * pl.row_tiles));
     s = std::min(s, ((long long)prefix_len + 127) / 128);

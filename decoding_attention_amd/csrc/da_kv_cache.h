@@ -14,8 +14,9 @@ struct KvPlane {
     int64_t page;                // elements between consecutive pages of the pool
     int dim;
     int aligned;                 // append: every 8 elements of src start at a multiple of 16 bytes
-    uint32_t lanes_magic;        // ceil(2^32 / (dim / 8)): chunk / (dim / 8) as one multiplication
-    uint32_t chunks_magic;       // ceil(2^32 / (head_k * dim / 8))
+    int narrow;                  // append: a work-group's offsets into src fit 24-bit products and 32-bit sums
+    uint32_t lanes_magic;        // ceil(2^32 / lanes of a row): chunk -> head as one multiplication
+    uint32_t chunks_magic;       // ceil(2^32 / chunks of a token)
 };
 
 struct KvCacheParams {

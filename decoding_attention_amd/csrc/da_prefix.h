@@ -7,11 +7,6 @@ namespace da {
 
 constexpr int kPrefixRows = 128;  // query rows of a prefix work-group: 32 for each of its four waves
 
-template <int D>
-constexpr int prefix_tile() {  // tokens of a K/V tile in LDS
-    return D <= 128 ? 64 : 32;
-}
-
 struct PrefixParams {
     SweepParams own;              // the sequences' own tokens; q, o, slopes, scale and head counts serve the prefix too
     const void* k;                // prefix rows [prefix_len, head_k, dim], or the page pools

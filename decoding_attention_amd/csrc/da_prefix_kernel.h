@@ -25,43 +25,49 @@
 namespace da {
 namespace prefix {
 
-// 16-byte chunk `c` of row `r` of a tile lies in slot swizzle(r, c) of the row: sixteen consecutive rows at one chunk (K),
-// and four rows at four consecutive chunks (V), fall into different banks.
+// A tile is 32 tokens.  Rows lie kPitch bytes apart and hold their 16-byte chunks XOR-swizzled with the row index, so that
+// sixteen consecutive rows at one chunk (K), and four rows at four consecutive chunks (V), fall into different banks.
+// (d = 96: twelve chunks and four empty ones, so that a load instruction fills whole rows here too.)
+constexpr int kTok = 32;
+constexpr int kEarlyExp = 10;  // exponentials of a tile taken beside the next one's score products
 template <int D>
-__device__ __forceinline__ int swizzle(int r, int c) {
-    if constexpr (D == 64) {  // two rows to the 256 bytes of the banks: bits 1 .. 3 of the row, reversed
-        return c ^ (((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1));
-    } else if constexpr (D == 96) {  // twelve chunks: no XOR stays inside the row
-        const int s = c + ((r >> 2) & 3);
-        return s >= 12 ? s - 12 : s;
-    } else {
-        return c ^ mla::swz_a(r);
-    }
+constexpr int pitch() {
+    return D == 96 ? 256 : D * 2;
 }
-// the row whose slot `s` this is holds chunk unswizzle(r, s) there
 template <int D>
-__device__ __forceinline__ int unswizzle(int r, int s) {
-    if constexpr (D == 96) {
-        const int c = s - ((r >> 2) & 3);
-        return c < 0 ? c + 12 : c;
-    } else {
-        return swizzle<D>(r, s);
-    }
+__device__ __forceinline__ int swizzle(int r) {
+    if constexpr (D == 64)  // two rows to the 256 bytes of the banks: bits 1 .. 3 of the row, reversed
+        return ((r >> 1) & 1) << 2 | ((r >> 2) & 1) << 1 | ((r >> 3) & 1);
+    else
+        return mla::swz_a(r);
 }
 
-template <typename Tag, int D>
+__device__ __forceinline__ auto join(s16x4_t lo, s16x4_t hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
+
+template <int D>
+constexpr size_t prefix_lds_bytes() {  // three buffers of K tiles and three of V tiles
+    return 6 * (size_t)kTok * pitch<D>();
+}
+
+// 16 bytes per lane from a wave-uniform address and a per-lane offset straight into LDS at `to` + lane * 16; the wait for it
+// is placed by hand.  (Plain loads: the row tiles of a split share its K/V through the L2.)
+__device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, uint32_t to) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(base), "s"(to) : "memory");
+}
+
+template <typename Tag, int D, int PGM>
 __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* const smem, const int hk, const int row0,
                                                const int split) {
     using MM = mla::Mma<Tag>;
     using EL = Elem<Tag>;
     using vec8 = typename MM::vec8;
-    constexpr int TT = prefix_tile<D>(), TB = TT / 32;
     constexpr int KS = D / 16, CB = D / 32;
-    constexpr int PITCH = D * 2, CPR = D / 8;
-    constexpr int TILE = TT * PITCH;           // bytes of a K (or V) tile
-    constexpr int LOADS = TILE / 4096;         // 1 KiB loads of a wave per tile and buffer
-    constexpr float kLazy = 8.0f;              // the running maximum moves only when exceeded by this much (log2 units)
-    static_assert(TILE % 4096 == 0, "whole loads");
+    constexpr int PITCH = pitch<D>(), SLOTS = PITCH / 16, CPR = D / 8;
+    constexpr int TILE = kTok * PITCH;   // bytes of a K (or V) tile
+    constexpr int LOADS = TILE / 4096;   // 1 KiB loads of a wave per tile
+    constexpr int RPL = 1024 / PITCH;    // rows of such a load
+    constexpr float kLazy = 8.0f;        // the running maximum moves only when exceeded by this much (log2 units)
+    static_assert(TILE % 4096 == 0 && 1024 % PITCH == 0, "whole loads of whole rows");
 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -69,6 +75,71 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
     const SweepParams& w = p.own;
 
     const int c0 = split * p.chunk, c1 = min(p.prefix_len, c0 + p.chunk);
+    const int last = c1 - 1, nu = (c1 - c0 + kTok - 1) / kTok;
+
+    // Tile loads: load i of a wave fills RPL rows, 16 bytes a lane, from a wave-uniform address and a per-lane offset.  PGM 0:
+    // the tile lies in one page (packed rows, or pages of 32 tokens and more); PGM 2: every load in one (pages of RPL tokens
+    // and more), or a look-up per lane (smaller ones).  Tokens past the split's end repeat its last one and are masked.
+    const int lrow = lane / SLOTS, slot = lane % SLOTS;
+    const uint32_t row_bytes = (uint32_t)w.k_row * 2;
+    uint32_t off[LOADS], off_end[LOADS];  // of any tile, and of the last one
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const int r = (wave * LOADS + i) * RPL + lrow;
+        const int c = slot ^ swizzle<D>(r);
+        const uint32_t col = (uint32_t)(c < CPR ? c : c - 8) * 16;  // (an empty chunk: any other one of the row)
+        off[i] = (uint32_t)r * row_bytes + col;
+        off_end[i] = (uint32_t)min(r, last - (c0 + (nu - 1) * kTok)) * row_bytes + col;
+    }
+    const uint8_t* const kbase = reinterpret_cast<const uint8_t*>(p.k) + (size_t)hk * D * 2;
+    const uint8_t* const vbase = reinterpret_cast<const uint8_t*>(p.v) + (size_t)hk * D * 2;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem + (uint32_t)(wave * LOADS) * 1024;
+    typedef const int32_t __attribute__((address_space(4))) * const_i32;
+    const const_i32 table = (const_i32)(uintptr_t)p.table;
+    const int page_mask = (1 << w.page_shift) - 1;
+    // bytes from the pool's (or the packed rows') start to token j, a wave-uniform one
+    auto row_at = [&](int j, int64_t page_stride) __attribute__((always_inline)) {
+        if (p.table == nullptr) return (int64_t)j * w.k_row * 2;
+        return ((int64_t)table[j >> w.page_shift] * page_stride + (int64_t)(j & page_mask) * w.k_row) * 2;
+    };
+    // END: the tile may be the last one (or lie behind it)
+    auto load = [&](const uint8_t* base, int64_t page_stride, int u, uint32_t to, auto end_c) __attribute__((always_inline)) {
+        constexpr bool END = decltype(end_c)::value;
+        if (END && u >= nu) return;
+        const int tok0 = c0 + u * kTok;
+        if constexpr (PGM == 0) {
+            const uint8_t* const at = base + row_at(tok0, page_stride);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) dma16(at, END && u == nu - 1 ? off_end[i] : off[i], lds0 + to + i * 1024);
+        } else if (page_mask + 1 >= RPL) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = (wave * LOADS + i) * RPL, j = END ? min(tok0 + r, last) : tok0 + r;
+                const uint32_t from = (uint32_t)(j - tok0) * row_bytes;
+                dma16(base + row_at(j, page_stride), (END && u == nu - 1 ? off_end[i] : off[i]) - from, lds0 + to + i * 1024);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const int r = (wave * LOADS + i) * RPL + lrow, j = min(tok0 + r, last);
+                const int64_t at = (int64_t)p.table[j >> w.page_shift] * page_stride + (int64_t)(j & page_mask) * w.k_row;
+                const uint32_t col = off[i] - (uint32_t)r * row_bytes;
+                mla::lds_dma16_v(base + at * 2 + col, lds0 + to + i * 1024);
+            }
+        }
+    };
+    auto load_k = [&](int u, int buf, auto end_c) __attribute__((always_inline)) { load(kbase, w.k_page, u, buf * TILE, end_c); };
+    auto load_v = [&](int u, int buf, auto end_c) __attribute__((always_inline)) {
+        load(vbase, w.v_page, u, (3 + buf) * TILE, end_c);
+    };
+    constexpr std::true_type kEnd{};
+    constexpr std::false_type kInner{};
+    load_k(0, 0, kEnd);
+    load_v(0, 0, kEnd);
+    load_k(1, 1, kEnd);
+    load_v(1, 1, kEnd);
+    load_k(2, 2, kEnd);
+
     // this lane's query row: number `row` among the KV head's; rows past the last one repeat it and are not stored
     const int row = row0 + wave * 32 + n;
     const bool live = row < p.rows;
@@ -79,47 +150,11 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) q[ks] = __builtin_bit_cast(vec8, *reinterpret_cast<const uint4*>(qrow + ks * 16 + h * 8));
     float slope = 0.0f;
-    int last = 0;  // position of the row's query token
+    int end = 0;  // position of the row's query token
     if (w.is_alibi) {
         slope = alibi_slope_log2(w.slopes, hq, w.head_q);
-        last = (p.table ? w.seq_lens[b] : p.prefix_len + w.cu_seq_k[b + 1] - w.cu_seq_k[b]) - 1;
+        end = (p.table ? w.seq_lens[b] : p.prefix_len + w.cu_seq_k[b + 1] - w.cu_seq_k[b]) - 1;
     }
-
-    // Tile loads: load i of a wave fills bytes [(wave * LOADS + i) KiB, + 1 KiB) of the tile, 16 bytes a lane; which row
-    // and chunk that is follows from the swizzle.  Tokens past the split's end repeat its last one and are masked.
-    int trow[LOADS], tcol[LOADS], page[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const int at = (wave * LOADS + i) * 64 + lane;  // 16-byte slot of the tile
-        trow[i] = at / CPR;
-        tcol[i] = unswizzle<D>(trow[i], at - trow[i] * CPR) * 8;
-    }
-    const uint16_t* const kbase = reinterpret_cast<const uint16_t*>(p.k) + (size_t)hk * D;
-    const uint16_t* const vbase = reinterpret_cast<const uint16_t*>(p.v) + (size_t)hk * D;
-    auto look_up = [&](int tok0) __attribute__((always_inline)) {
-        if (p.table == nullptr) return;
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) page[i] = p.table[min(tok0 + trow[i], c1 - 1) >> w.page_shift];
-    };
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-    auto load = [&](int tok0, uint32_t buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            const int tok = min(tok0 + trow[i], c1 - 1);
-            int64_t ko, vo;
-            if (p.table == nullptr) {
-                ko = (int64_t)tok * w.k_row + tcol[i];
-                vo = ko;
-            } else {
-                const int64_t in = (int64_t)(tok & ((1 << w.page_shift) - 1)) * w.k_row + tcol[i];
-                ko = (int64_t)page[i] * w.k_page + in;
-                vo = (int64_t)page[i] * w.v_page + in;
-            }
-            const uint32_t to = buf + (wave * LOADS + i) * 1024;
-            mla::lds_dma16_v(kbase + ko, to);
-            mla::lds_dma16_v(vbase + vo, to + TILE);
-        }
-    };
 
     f32x16 acc[CB];
 #pragma unroll
@@ -128,64 +163,51 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         for (int i = 0; i < 16; ++i) acc[cb][i] = 0.0f;
     float m = kNegBig, l = 0.0f;
 
-    // LDS addresses of this lane: K row n (+ 32 per block) at every k-step, V^T of rows 4 h + (lane >> 2 & 3)
-    const uint8_t* const tile0 = smem;
-    const int vr = h * 4 + ((lane >> 2) & 3);
-    const int vcol = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;  // first of the lane's four columns in a block of 32
-
-    look_up(c0);
-    load(c0, lds0);
-    look_up(min(c0 + TT, c1 - 1));
-    const int ntiles = (c1 - c0 + TT - 1) / TT;
-    for (int t = 0; t < ntiles; ++t) {
-        const int tok0 = c0 + t * TT;
-        // this wave's share of tile t has landed and its reads of tile t - 1 are done; after the barrier, everyone's
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + 1 < ntiles) {
-            load(tok0 + TT, lds0 + ((t + 1) & 1) * (2 * TILE));
-            look_up(min(tok0 + 2 * TT, c1 - 1));
+    // LDS offsets of this lane: K row n at every k-step; V rows 4 h + (lane >> 2 & 3) and eight further down, four columns
+    // of every block of 32
+    int k_at[KS], v_at[CB][2];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k_at[ks] = n * PITCH + ((ks * 2 + h) ^ swizzle<D>(n)) * 16;
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = h * 4 + ((lane >> 2) & 3) + 8 * j, c = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+            v_at[cb][j] = r * PITCH + ((cb * 4 + (c >> 3)) ^ swizzle<D>(r)) * 16 + (c & 4) * 2;
         }
-        const uint8_t* const kt = tile0 + (t & 1) * (2 * TILE);
-        const uint8_t* const vt = kt + TILE;
 
-        f32x16 s[TB];
+    // The score tile of 32 tokens: element i is token 8 (i / 4) + 4 h + i % 4 of the tile, row n.
+    f32x16 s;
+    float mul = w.scale_log2;  // what takes s to log2 units
+    auto scores = [&](const vec8(&kf)[KS]) __attribute__((always_inline)) {
+        f32x16 c;
 #pragma unroll
-        for (int tb = 0; tb < TB; ++tb) {
+        for (int i = 0; i < 16; ++i) c[i] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[tb][i] = 0.0f;
+        for (int ks = 0; ks < KS; ++ks) c = MM::mma(kf[ks], q[ks], c);
+        return c;
+    };
+    auto max_of = [](const f32x16& x) __attribute__((always_inline)) {
+        float mx = x[0];
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const int r = tb * 32 + n;
-                const vec8 kf = *reinterpret_cast<const vec8*>(kt + r * PITCH + swizzle<D>(r, ks * 2 + h) * 16);
-                s[tb] = MM::mma(kf, q[ks], s[tb]);
+        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+        return mx;
+    };
+    // ALiBi and the mask of tokens past the end, the running maximum, and (rarely) the rescaling it asks for; mx: max_of(s)
+    auto settle_max = [&](int u, float mx) __attribute__((always_inline)) {
+        const int tok0 = c0 + u * kTok;
+        if (w.is_alibi || tok0 + kTok > c1) {
+            const float at = (float)(tok0 + 4 * h - end);  // (whole numbers below 2^24: exact)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = (i >> 2) * 8 + (i & 3);
+                const float x = s[i] * w.scale_log2 + slope * (at + (float)j);
+                s[i] = tok0 + 4 * h + j >= c1 ? -INFINITY : x;
             }
+            mul = 1.0f;
+            mx = max_of(s);
         }
-
-        // x = score in log2 units; element i of block tb is token tok0 + 32 tb + 8 (i / 4) + 4 h + i % 4
-        const bool tail = tok0 + TT > c1;
-        if (w.is_alibi || tail) {
-            const float at = (float)(tok0 + 4 * h - last);  // (whole numbers below 2^24: exact)
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = tb * 32 + (i >> 2) * 8 + (i & 3);
-                    float x = s[tb][i] * w.scale_log2 + slope * (at + (float)j);
-                    if (tok0 + 4 * h + j >= c1) x = -INFINITY;
-                    s[tb][i] = x;
-                }
-        } else {
-#pragma unroll
-            for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[tb][i] *= w.scale_log2;
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[tb][i]);
-        mx = max_xor32(mx);
+        mx = max_xor32(mx) * mul;
         const bool up = mx > m + kLazy;
         if (__any(up)) {
             const float mn = up ? mx : m;
@@ -195,37 +217,102 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) acc[cb] *= alpha;
         }
-        vec8 pf[TB * 2];
-        constexpr uint32_t kOnes = std::is_same<Tag, f16_tag>::value ? 0x3C003C00u : 0x3F803F80u;
+    };
+    auto k_fragments = [&](int buf, vec8(&kf)[KS]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-            for (int kk = 0; kk < 2; ++kk) {
-                uint32_t pw[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float lo = fast_exp2(s[tb][kk * 8 + 2 * j] - m), hi = fast_exp2(s[tb][kk * 8 + 2 * j + 1] - m);
-                    pw[j] = EL::pack2(lo, hi);
-                    // (the denominator sums the probabilities as the second product sees them)
-                    l = EL::dot2(pw[j], kOnes, l);
-                }
-                pf[tb * 2 + kk] = __builtin_bit_cast(vec8, make_uint4(pw[0], pw[1], pw[2], pw[3]));
-            }
+        for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const vec8*>(smem + buf * TILE + k_at[ks]);
+    };
 
-        typedef __attribute__((address_space(3))) s16x4_t* lds_s4;
-#pragma unroll
-        for (int k = 0; k < TB * 2; ++k) {
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                const int r0 = k * 16 + vr, r1 = r0 + 8, c = cb * 4 + (vcol >> 3), in = (vcol & 4) * 2;
-                const s16x4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s4)(vt + r0 * PITCH + swizzle<D>(r0, c) * 16 + in));
-                const s16x4_t d = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (lds_s4)(vt + r1 * PITCH + swizzle<D>(r1, c) * 16 + in));
-                const s16x8_t both = __builtin_shufflevector(a, d, 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[cb] = MM::mma(__builtin_bit_cast(vec8, both), pf[k], acc[cb]);
-            }
+    // One tile: the score products of the next one beside this one's exponentials, then its value products beside the
+    // next one's maximum.
+    auto step = [&](int u, auto buf_c) __attribute__((always_inline)) {
+        constexpr int buf = decltype(buf_c)::value, next = (buf + 1) % 3, prev = (buf + 2) % 3;
+        // K of tile u + 1 and V of tile u have landed (this wave's share; after the barrier, everyone's), and the reads of
+        // K(u) and V(u - 1), whose buffers are filled next, are done
+        if (u + 4 < nu) {
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            load_k(u + 3, buf, kInner);
+            load_v(u + 2, prev, kInner);
+        } else {
+            if (u + 2 < nu)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            else
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            load_k(u + 3, buf, kEnd);
+            load_v(u + 2, prev, kEnd);
         }
+        // From here to the maximum the order of issue is the source's: one matrix instruction occupies its unit for 32
+        // cycles, in whose shadow go an exponential or two (16 cycles each) and the LDS reads of what comes later.
+        vec8 kf[KS];
+        k_fragments(next, kf);  // (past the last tile: of whatever lies there, not used)
+        typedef __attribute__((address_space(3))) s16x4_t* lds_s4;
+        uint8_t* const vt = smem + (3 + buf) * TILE;
+        s16x4_t vf[2][CB][2];
+        auto read_v = [&](int i) __attribute__((always_inline)) {  // i-th of the 4 CB reads
+            const int kk = i / (2 * CB), cb = i / 2 % CB, j = i % 2;
+            vf[kk][cb][j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(vt + kk * 16 * PITCH + v_at[cb][j]));
+        };
+        float e[16];
+        uint32_t pw[8];
+        constexpr uint32_t kOnes = std::is_same<Tag, f16_tag>::value ? 0x3C003C00u : 0x3F803F80u;
+        auto exponential = [&](int i) __attribute__((always_inline)) {
+            e[i] = fast_exp2(__builtin_fmaf(s[i], mul, -m));
+            if (i & 1) pw[i / 2] = EL::pack2(e[i - 1], e[i]);
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 s_next;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s_next[i] = 0.0f;
+        static_for<0, KS>([&](auto ks_c) __attribute__((always_inline)) {
+            constexpr int ks = decltype(ks_c)::value;
+            s_next = MM::mma(kf[ks], q[ks], s_next);
+            constexpr int e0 = kEarlyExp * ks / KS, e1 = kEarlyExp * (ks + 1) / KS;
+#pragma unroll
+            for (int i = e0; i < e1; ++i) exponential(i);
+#pragma unroll
+            for (int i = 4 * CB * ks / KS; i < 4 * CB * (ks + 1) / KS; ++i) read_v(i);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        static_for<0, CB>([&](auto cb_c) __attribute__((always_inline)) {
+            constexpr int cb = decltype(cb_c)::value;
+            const vec8 pf = __builtin_bit_cast(vec8, make_uint4(pw[0], pw[1], pw[2], pw[3]));
+            acc[cb] = MM::mma(__builtin_bit_cast(vec8, join(vf[0][cb][0], vf[0][cb][1])), pf, acc[cb]);
+            constexpr int n_exp = 16 - kEarlyExp;
+#pragma unroll
+            for (int i = kEarlyExp + n_exp * cb / CB; i < kEarlyExp + n_exp * (cb + 1) / CB; ++i) exponential(i);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        float mx = s_next[0];
+        static_for<0, CB>([&](auto cb_c) __attribute__((always_inline)) {
+            constexpr int cb = decltype(cb_c)::value;
+            const vec8 pf = __builtin_bit_cast(vec8, make_uint4(pw[4], pw[5], pw[6], pw[7]));
+            acc[cb] = MM::mma(__builtin_bit_cast(vec8, join(vf[1][cb][0], vf[1][cb][1])), pf, acc[cb]);
+            // (the denominator sums the probabilities as the second product sees them)
+#pragma unroll
+            for (int j = 8 * cb / CB; j < 8 * (cb + 1) / CB; ++j) l = EL::dot2(pw[j], kOnes, l);
+#pragma unroll
+            for (int i = 16 * cb / CB; i < 16 * (cb + 1) / CB; ++i) mx = fmaxf(mx, s_next[i]);
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        s = s_next;
+        if (u + 1 < nu) settle_max(u + 1, mx);
+    };
+
+    // the first tile's scores
+    if (nu > 2)
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * LOADS) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    {
+        vec8 kf[KS];
+        k_fragments(0, kf);
+        s = scores(kf);
+    }
+    settle_max(0, max_of(s));
+    for (int u = 0; u < nu; u += 3) {
+        step(u, std::integral_constant<int, 0>{});
+        if (u + 1 < nu) step(u + 1, std::integral_constant<int, 1>{});
+        if (u + 2 < nu) step(u + 2, std::integral_constant<int, 2>{});
     }
 
     l += __shfl_xor(l, 32);
@@ -252,7 +339,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         const int g = rest * 8 + (id & 7);  // (KV head, split)
         if (g >= p.own.head_k * p.splits) return;
         const int split = g / p.own.head_k;
-        prefix_segment<Tag, D>(p, smem, g - split * p.own.head_k, (slot - rest * p.row_tiles) * kPrefixRows, split);
+        prefix_segment<Tag, D, PGM>(p, smem, g - split * p.own.head_k, (slot - rest * p.row_tiles) * kPrefixRows, split);
         return;
     }
     const SweepParams& w = p.own;
@@ -279,7 +366,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
 
 template <typename Tag, int D, bool WH, int PGM>
 hipError_t launch_form(const PrefixParams& p, int own_wgs, hipStream_t stream) {
-    constexpr size_t tiles = 4 * (size_t)prefix_tile<D>() * D * 2, segment = gqa_lds_bytes<D>(1);
+    constexpr size_t tiles = prefix_lds_bytes<D>(), segment = gqa_lds_bytes<D>(1);
     constexpr size_t lds = tiles > segment ? tiles : segment;
     auto kern = prefix_kernel<Tag, D, WH, PGM>;
     if (lds > 48 * 1024) {
