@@ -49,10 +49,13 @@ int env_int(const char* name, int dflt) {
 struct Tunables {
     int target_wgs, mfma_target_wgs, max_chunk, min_chunk, ragged_chunk, force_kind, group_min_ratio, wave_per_head,
         mla_heads, gqa_heads, flat_wgs, flat_min_tokens, flat_uncounted, flat_uncounted_min, flat_paged_min_mb, nsplit, mfma_small_wgs, group_small_wgs,
-        group_small_chunk, mla_group_heads, mla_group_small, fill_rounds, group_target_wgs_d128, mla_distinct_v;
+        group_small_chunk, mla_group_heads, mla_group_small, fill_rounds, group_target_wgs_d128, mla_distinct_v, prefix_own_wgs,
+        prefix_splits;
     Tunables() {
         target_wgs = env_int("DA_TARGET_WGS", 512);
         mfma_target_wgs = env_int("DA_MFMA_TARGET_WGS", 256);
+        prefix_own_wgs = env_int("DA_PREFIX_OWN_WGS", 256);
+        prefix_splits = env_int("DA_PREFIX_SPLITS", 0);
         max_chunk = env_int("DA_MAX_CHUNK", 1024);
         min_chunk = env_int("DA_MIN_CHUNK", 512);
         gqa_heads = env_int("DA_GQA_HEADS", 0);  // query heads per work-group and KV head of the grouped kernel (16/32), 0 = by shape
@@ -1399,45 +1402,93 @@ struct PrefixPlan {
     bool wave_per_head = false;
     int row_tiles = 0, splits = 0, chunk = 0, prefix_wgs = 0;
     int groups = 0, own_splits = 0, own_chunk = 1, own_groups = 0;
+    int flat_wgs = 0, flat_step = 1, flat_min = 1, flat_unit = 1;  // balanced own part (see Plan)
+    bool scan = false;
     long long own_wgs = 0;
     size_t prefix_parts = 0, own_parts = 0;  // partial rows of either part
-    size_t ws_bytes = 0;
+    size_t flat_cu_bytes = 0, ws_bytes = 0;
 };
 
-// own_max: most own tokens of a sequence.
-PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t batch, size_t head_q, size_t head_k, size_t dim) {
+// own_max: most own tokens of a sequence; own_total: all own tokens, 0 = unknown.
+PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total, size_t batch, size_t head_q, size_t head_k,
+                            size_t dim, size_t page_size) {
     PrefixPlan pl;
     const long long ratio = (long long)(head_q / head_k), rows = (long long)batch * ratio;
-    const long long tile = 32;
-    pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
-    long long s = std::max<long long>(1, 256 / ((long long)head_k * pl.row_tiles));
-    s = std::min(s, ((long long)prefix_len + 127) / 128);
-    long long chunk = ((long long)prefix_len + s - 1) / s;
-    chunk = (chunk + tile - 1) / tile * tile;
-    pl.chunk = (int)chunk;
-    pl.splits = (int)(((long long)prefix_len + chunk - 1) / chunk);
-    pl.prefix_wgs = (int)(((long long)head_k * pl.splits + 7) / 8 * 8 * pl.row_tiles);
-    pl.prefix_parts = (size_t)pl.splits * batch * head_q;
+    if (own_total == 0 || own_total > batch * own_max) own_total = batch * own_max;
 
     pl.wave_per_head = head_k % 4 == 0;
     pl.groups = (int)((ratio + 15) / 16);
     pl.own_groups = (int)(pl.wave_per_head ? head_k / 4 : head_k) * pl.groups;
     if (own_max > 0) {
         const long long trip = pl.wave_per_head ? da::kGqaTile : 4 * da::kGqaTile;
-        const long long base = (long long)batch * pl.own_groups;
-        long long ns = std::max<long long>(1, 512 / base);
-        ns = std::max(ns, ((long long)own_max + 1023) / 1024);
-        ns = std::min(ns, ((long long)own_max + trip - 1) / trip);
-        long long oc = ((long long)own_max + ns - 1) / ns;
-        oc = (oc + trip - 1) / trip * trip;
-        pl.own_chunk = (int)oc;
-        pl.own_splits = (int)(((long long)own_max + oc - 1) / oc);
-        const long long segs = (long long)batch * pl.own_splits * (pl.own_groups / pl.groups);
+        const long long target = tun().prefix_own_wgs * (dim == 64 ? 2 : 1), shares = std::max<long long>(1, target / pl.own_groups);
+        // equal shares where every one gets 128 tokens and more: 256 sequences of 0 .. 1024 own tokens, 32/8 heads d 128, 102 us
+        // where splits of 1024 tokens take 145
+        const long long unit = page_size == 0 ? 1 : da::kGqaTile;
+        if ((long long)own_total >= 128 * shares && (page_size == 0 || batch <= (size_t)da::kScanBatch) &&
+            batch * own_max < ((size_t)1 << 30) && tun().flat_wgs > 0) {
+            pl.flat_wgs = (int)shares;
+            pl.flat_unit = (int)unit;
+            pl.flat_step = (int)std::max<long long>(1, trip / unit);
+            pl.flat_min = (int)std::max<long long>(128 / unit, pl.flat_step);
+            pl.scan = page_size != 0;
+            pl.own_parts = da::flat_slots(pl.flat_wgs, batch) * head_q;
+            pl.own_splits = 1;
+            pl.own_chunk = (int)trip;
+            if (pl.scan) pl.flat_cu_bytes = ((batch + 1) * sizeof(int32_t) + 15) / 16 * 16;
+        } else {
+            const long long base = (long long)batch * pl.own_groups;
+            long long ns = std::max<long long>(1, 512 / base);
+            ns = std::max(ns, ((long long)own_max + 1023) / 1024);
+            ns = std::min(ns, ((long long)own_max + trip - 1) / trip);
+            long long oc = ((long long)own_max + ns - 1) / ns;
+            oc = (oc + trip - 1) / trip * trip;
+            pl.own_chunk = (int)oc;
+            pl.own_splits = (int)(((long long)own_max + oc - 1) / oc);
+            pl.own_parts = (size_t)pl.own_splits * batch * head_q;
+        }
+        const long long segs =
+            (pl.flat_wgs ? (long long)pl.flat_wgs : (long long)batch * pl.own_splits) * (pl.own_groups / pl.groups);
         pl.own_wgs = pl.groups > 1 ? (segs + 7) / 8 * 8 * pl.groups : segs;
-        pl.own_parts = (size_t)pl.own_splits * batch * head_q;
     }
-    pl.ws_bytes = (pl.prefix_parts + pl.own_parts) * (dim + 2) * sizeof(float);
+
+    // Splits of the prefix: the least of (the longer of both parts' times) + (the partials' way out and back).  A work-group
+    // takes 10 us and about 0.0052 us per (tile, column); one runs on a CU beside an own one (d = 256: alone), two where the own
+    // tokens are few; the (KV head, split) pairs are dealt out over the eight XCDs.
+    pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
+    const double own_us = 4.0 * (double)own_total * (double)head_k * (double)dim / 5.0e6 + (own_max > 0 ? 6.0 : 0.0);
+    double best = 0.0;
+    long long best_s = 1;
+    const long long most = std::min<long long>(((long long)prefix_len + 63) / 64, 64);
+    for (long long s = 1; s <= most; ++s) {
+        const long long tiles = ((long long)prefix_len + 32 * s - 1) / (32 * s);
+        const long long per_xcd = ((long long)head_k * s + 7) / 8 * pl.row_tiles;
+        const double part_us = 2.0 * 4.0 * (double)s * (double)batch * (double)head_q * (double)(dim + 2) / 4.0e6;
+        for (int pair = 0; pair < (dim <= 128 ? 2 : 1); ++pair) {
+            const double step = 0.0052 * (double)dim * (pair ? 1.4 : 1.0);
+            const double us = 10.0 + (double)((per_xcd + 32 * (pair + 1) - 1) / (32 * (pair + 1))) * (double)tiles * step;
+            const double cost = (pair ? us + own_us : std::max(us, own_us)) + part_us;
+            if (best == 0.0 || cost < best) {
+                best = cost;
+                best_s = s;
+            }
+        }
+    }
+    if (tun().prefix_splits > 0) best_s = std::min<long long>(tun().prefix_splits, most);
+    long long chunk = ((long long)prefix_len + best_s - 1) / best_s;
+    chunk = (chunk + 31) / 32 * 32;
+    pl.chunk = (int)chunk;
+    pl.splits = (int)(((long long)prefix_len + chunk - 1) / chunk);
+    pl.prefix_wgs = (int)(((long long)head_k * pl.splits + 7) / 8 * 8 * pl.row_tiles);
+    pl.prefix_parts = (size_t)pl.splits * batch * head_q;
+    pl.ws_bytes = (pl.prefix_parts + pl.own_parts) * (dim + 2) * sizeof(float) + pl.flat_cu_bytes;
     return pl;
+}
+
+// A paged call's count is that of whole sequences; padded rows of the batch hold none, so what the prefix takes off is a guess
+// (a hint as everywhere: it only moves the plan).
+size_t own_tokens(size_t total_k, size_t prefix_len, size_t batch) {
+    return total_k == 0 ? 0 : (total_k > prefix_len * batch ? total_k - prefix_len * batch : total_k % prefix_len);
 }
 
 int check_prefix_shape(size_t prefix_len, size_t max_seq_k, size_t batch, size_t head_q, size_t head_k, size_t dim,
@@ -1457,7 +1508,7 @@ int check_prefix_shape(size_t prefix_len, size_t max_seq_k, size_t batch, size_t
 
 // table: page ids of the prefix (paged), else null and pk, pv are the prefix's packed rows.
 int run_shared_prefix(const void* q, const void* pk, const void* pv, const int32_t* table, size_t prefix_len, const void* k,
-                      const void* v, void* o, const int32_t* cu_seq_k, const Paging& pg, size_t own_max, size_t batch,
+                      const void* v, void* o, const int32_t* cu_seq_k, const Paging& pg, size_t own_max, size_t own_total, size_t batch,
                       size_t head_q, size_t head_k, size_t dim, int is_alibi, int is_bf16, float softmax_scale,
                       const float* alibi_slopes, void* workspace, size_t workspace_bytes, void* hip_stream) {
     if (!q) return fail(DA_ERR_INVALID_ARGUMENT, "q is null");
@@ -1467,7 +1518,7 @@ int run_shared_prefix(const void* q, const void* pk, const void* pv, const int32
     if (!aligned16(q) || !aligned16(pk) || !aligned16(pv) || !aligned16(k) || !aligned16(v) || !aligned16(o))
         return fail(DA_ERR_INVALID_ARGUMENT, "q, o and all K and V must be 16-byte aligned");
     if (batch == 0) return DA_OK;
-    const PrefixPlan pl = make_prefix_plan(prefix_len, own_max, batch, head_q, head_k, dim);
+    const PrefixPlan pl = make_prefix_plan(prefix_len, own_max, own_total, batch, head_q, head_k, dim, pg.table ? pg.page_size : 0);
     if (pl.prefix_wgs + pl.own_wgs > (long long)INT32_MAX / 2)
         return fail(DA_ERR_INVALID_ARGUMENT, "shape out of range (%lld work-groups)", pl.prefix_wgs + pl.own_wgs);
     hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
@@ -1493,6 +1544,13 @@ int run_shared_prefix(const void* q, const void* pk, const void* pv, const int32
     w.ws_o = take(pl.own_parts * dim);
     p.ws_ml = take(pl.prefix_parts * 2);
     w.ws_ml = take(pl.own_parts * 2);
+    p.scan = pl.scan ? 1 : 0;
+    p.flat_out = pl.scan ? reinterpret_cast<int32_t*>(static_cast<uint8_t*>(ws) + (pl.ws_bytes - pl.flat_cu_bytes)) : nullptr;
+    w.flat_wgs = pl.flat_wgs;
+    w.flat_step = pl.flat_step;
+    w.flat_min = pl.flat_min;
+    w.flat_unit = pl.flat_unit;
+    w.flat_cu = pl.scan ? p.flat_out : cu_seq_k;
     p.k = pk;
     p.v = pv;
     p.table = table;
@@ -1557,8 +1615,8 @@ int da_decoding_attn_shared_prefix(const void* q, const void* k_prefix, const vo
         return run_attention(q, k, v, o, cu_seq_k, Paging{}, KvFormat{}, max_seq_k, batch, head_q, head_k, dim, dim_v,
                              is_alibi, is_bf16, softmax_scale, alibi_slopes, total_k, workspace, workspace_bytes, hip_stream);
     }
-    return run_shared_prefix(q, k_prefix, v_prefix, nullptr, prefix_len, k, v, o, cu_seq_k, Paging{}, max_seq_k, batch, head_q,
-                             head_k, dim, is_alibi, is_bf16, softmax_scale, alibi_slopes, workspace, workspace_bytes,
+    return run_shared_prefix(q, k_prefix, v_prefix, nullptr, prefix_len, k, v, o, cu_seq_k, Paging{}, max_seq_k, total_k, batch,
+                             head_q, head_k, dim, is_alibi, is_bf16, softmax_scale, alibi_slopes, workspace, workspace_bytes,
                              hip_stream);
 }
 
@@ -1584,7 +1642,8 @@ int da_decoding_attn_paged_shared_prefix(const void* q, const void* k_pages, con
         return fail(DA_ERR_INVALID_ARGUMENT, "prefix_len (%zu) must be a multiple of page_size (%zu): whole pages are shared",
                     prefix_len, page_size);
     return run_shared_prefix(q, k_pages, v_pages, prefix_blocks, prefix_len, k_pages, v_pages, o, nullptr, pg,
-                             max_seq_k > prefix_len ? max_seq_k - prefix_len : 0, batch, head_q, head_k, dim, is_alibi, is_bf16,
+                             max_seq_k > prefix_len ? max_seq_k - prefix_len : 0, own_tokens(total_k, prefix_len, batch), batch,
+                             head_q, head_k, dim, is_alibi, is_bf16,
                              softmax_scale, alibi_slopes, workspace, workspace_bytes, hip_stream);
 }
 
@@ -1593,7 +1652,9 @@ size_t da_workspace_bytes_shared_prefix(size_t prefix_len, size_t max_seq_k, siz
     if (head_k == 0 || head_q % head_k != 0 || !supported_dims(dim, dim_v) || dim != dim_v || batch == 0) return 0;
     if (prefix_len == 0) return plan_ws_bytes(max_seq_k, batch, head_q, head_k, dim, dim_v, true, total_k, page_size);
     const size_t own = page_size == 0 ? max_seq_k : (max_seq_k > prefix_len ? max_seq_k - prefix_len : 0);
-    return make_prefix_plan(prefix_len, own, batch, head_q, head_k, dim).ws_bytes;
+    return make_prefix_plan(prefix_len, own, page_size == 0 ? total_k : own_tokens(total_k, prefix_len, batch), batch, head_q,
+                            head_k, dim, page_size)
+        .ws_bytes;
 }
 
 }  // extern "C"

@@ -6,6 +6,7 @@
 namespace da {
 
 constexpr int kPrefixRows = 128;  // query rows of a prefix work-group: 32 for each of its four waves
+constexpr int kScanBatch = 1024;  // most sequences whose lengths a work-group adds up in LDS
 
 struct PrefixParams {
     SweepParams own;              // the sequences' own tokens; q, o, slopes, scale and head counts serve the prefix too
@@ -16,7 +17,9 @@ struct PrefixParams {
     int rows, row_tiles;          // query rows per KV head (batch * ratio), in tiles of kPrefixRows
     int splits, chunk;            // prefix splits and tokens per split (a multiple of the tile)
     int prefix_wgs;               // work-groups in front of own's: 8 * ceil(head_k * splits / 8) * row_tiles
-    int own_groups;               // own's work-groups per sequence and split: (head_k or head_k / 4) * own.groups
+    int own_groups;               // own's work-groups per segment: (head_k or head_k / 4) * own.groups
+    int scan;                     // balanced own part over pages: the kernel adds the lengths up itself (flat_cu is written)
+    int32_t* flat_out;            // [batch + 1] (scan)
     float* ws_o;                  // [splits, batch * head_q, dim] un-normalised partial outputs
     float* ws_ml;                 // [splits, batch * head_q, 2] running maximum (log2 units) and denominator
 };

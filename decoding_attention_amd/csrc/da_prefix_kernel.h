@@ -328,8 +328,49 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
     if (h == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(m, l);
 }
 
+// Own tokens of sequence b (paged sequences count the prefix in their lengths).
+__device__ __forceinline__ int own_len(const PrefixParams& p, int b) {
+    return p.table ? max(p.own.seq_lens[b] - p.prefix_len, 0) : p.own.cu_seq_k[b + 1] - p.own.cu_seq_k[b];
+}
+
+// Positions of the sequences on the balanced grid's line, in units of flat_unit tokens (every sequence rounded up), into LDS:
+// at[0 .. batch].  Thread t adds up sequences 4 t .. 4 t + 3.
+__device__ __forceinline__ void scan_lengths(const PrefixParams& p, int32_t* at) {
+    const SweepParams& w = p.own;
+    int n[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int b = (int)threadIdx.x * 4 + i;
+        n[i] = sum;
+        if (b < w.batch) sum += (own_len(p, b) + w.flat_unit - 1) / w.flat_unit;
+    }
+    int incl = sum;
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(incl, d);
+        if (lane >= d) incl += other;
+    }
+    int32_t* const waves = at + kScanBatch + 1;
+    if (lane == 63) waves[threadIdx.x >> 6] = incl;
+    __syncthreads();
+    int base = incl - sum;
+    for (int i = 0; i < (int)(threadIdx.x >> 6); ++i) base += waves[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int b = (int)threadIdx.x * 4 + i;
+        if (b <= w.batch) at[b] = base + n[i];
+    }
+    if (threadIdx.x == 255 && w.batch == kScanBatch) at[kScanBatch] = base + sum;
+    __syncthreads();
+}
+constexpr size_t kScanBytes = (kScanBatch + 1 + 4) * sizeof(int32_t);
+
 // Work-groups are numbered so that the row tiles of one (KV head, prefix split) run on one XCD (consecutive work-groups go
 // to the eight XCDs in turn) and share its K/V through that XCD's L2; likewise the head groups of one own-token segment.
+//
+// The own tokens are cut in one of two ways, as in the grouped kernel: own.flat_wgs == 0: (sequence, split of own.chunk tokens);
+// else the sequences' tokens form one line, and each of flat_wgs shares of it is one work-group's (per KV heads and group).
 template <typename Tag, int D, bool WH, int PGM>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prefix_kernel(const PrefixParams p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -352,44 +393,90 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     }
     const int ny = p.own_groups / w.groups;
     const int by = (seg % ny) * w.groups + grp;
-    const int rest = seg / ny;
-    const int split = rest % w.nsplit, b = rest / w.nsplit;
-    if (b >= w.batch) return;  // (the last eight of several head groups)
-    int start, len;
-    seq_range(w, b, start, len);
-    const int own0 = p.table ? p.prefix_len : 0;  // paged: the sequence's positions count the prefix
-    const int c0 = own0 + split * w.chunk;
-    const int c1 = split == w.nsplit - 1 ? len : min(len, c0 + w.chunk);
-    gqa_segment<Tag, D, D, 1, (D <= 256), WH, 0, PGM>(p.own, smem, by, b, start, len, c0, c1,
-                                                      (size_t)b * w.head_q * w.nsplit + split, w.nsplit, false);
+    const int own0 = p.table ? p.prefix_len : 0;
+    // which tokens: the balanced grid's share, or split number `split` of one sequence
+    const int32_t* cu = w.flat_cu;
+    int b = 0, r0 = 0, r1 = 0, share = 0, split = 0;
+    if (w.flat_wgs > 0) {
+        share = seg / ny;
+        if (share >= w.flat_wgs) return;
+        if (p.scan) {
+            int32_t* const at = reinterpret_cast<int32_t*>(smem + gqa_lds_bytes<D>(1));
+            scan_lengths(p, at);
+            if (share == 0 && by == 0)  // (for the merge)
+                for (int j = threadIdx.x; j <= w.batch; j += 256) p.flat_out[j] = at[j];
+            cu = at;
+        }
+        const int total = cu[w.batch];
+        const int T = flat_share(total, w.flat_wgs, w.flat_step, w.flat_min);
+        r0 = (int)min((long long)share * T, (long long)total);
+        r1 = share == w.flat_wgs - 1 ? total : (int)min((long long)r0 + T, (long long)total);
+        if (r0 >= r1) return;
+        for (int n = w.batch; n > 1;) {  // the last b with cu[b] <= r0: 64 probes at once
+            const int stride = (n + 63) >> 6;
+            const int idx = b + (int)(threadIdx.x & 63) * stride;
+            const int k = __popcll(__ballot(idx < b + n && cu[idx] <= r0)) - 1;
+            b += k * stride;
+            n = min(stride, n - k * stride);
+        }
+    } else {
+        split = (seg / ny) % w.nsplit;
+        b = seg / ny / w.nsplit;
+        if (b >= w.batch) return;  // (the last eight of several head groups)
+    }
+    for (;; ++b) {
+        int start, len, c0, c1;
+        size_t part0;
+        if (w.flat_wgs > 0) {
+            if (b >= w.batch) break;
+            const int s = cu[b], e = cu[b + 1];
+            if (s >= r1) break;
+            if (e <= s) continue;
+            seq_range(w, b, start, len);
+            c0 = own0 + (max(r0, s) - s) * w.flat_unit;
+            c1 = min(own0 + (min(r1, e) - s) * w.flat_unit, len);
+            part0 = (size_t)(share + b) * w.head_q;
+        } else {
+            seq_range(w, b, start, len);
+            c0 = own0 + split * w.chunk;
+            c1 = split == w.nsplit - 1 ? len : min(len, c0 + w.chunk);
+            part0 = (size_t)b * w.head_q * w.nsplit + split;
+        }
+        gqa_segment<Tag, D, D, 1, true, WH, 0, PGM>(p.own, smem, by, b, start, len, c0, c1, part0, w.flat_wgs > 0 ? 1 : w.nsplit,
+                                                    false);
+        if (w.flat_wgs == 0) break;
+        if (!WH) __syncthreads();  // the merge area of this segment is the V tile area of the next
+    }
 }
 
 template <typename Tag, int D, bool WH, int PGM>
 hipError_t launch_form(const PrefixParams& p, int own_wgs, hipStream_t stream) {
-    constexpr size_t tiles = prefix_lds_bytes<D>(), segment = gqa_lds_bytes<D>(1);
-    constexpr size_t lds = tiles > segment ? tiles : segment;
+    const size_t segment = gqa_lds_bytes<D>(1) + (p.scan ? kScanBytes : 0);
+    const size_t lds = prefix_lds_bytes<D>() > segment ? prefix_lds_bytes<D>() : segment;
     auto kern = prefix_kernel<Tag, D, WH, PGM>;
     if (lds > 48 * 1024) {
         static std::atomic<uint64_t> devices_done{0};
-        const hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(kern), lds, devices_done);
+        const hipError_t e = ensure_lds_limit(reinterpret_cast<const void*>(kern), 160 * 1024, devices_done);
         if (e != hipSuccess) return e;
     }
     hipLaunchKernelGGL(kern, dim3((unsigned)(p.prefix_wgs + own_wgs)), dim3(256), lds, stream, p);
     return hipGetLastError();
 }
 
+template <typename Tag, int D, bool WH>
+hipError_t launch_pages(const PrefixParams& p, int own_wgs, hipStream_t stream) {
+    // how a tile's rows are found: whole tiles in pages of 32 tokens and more (and packed rows), two runs in 16-token pages,
+    // a look-up for every row in smaller ones
+    if (p.own.block_table == nullptr || p.own.page_shift >= 5) return launch_form<Tag, D, WH, 0>(p, own_wgs, stream);
+    if (p.own.page_shift == 4) return launch_form<Tag, D, WH, 1>(p, own_wgs, stream);
+    return launch_form<Tag, D, WH, 2>(p, own_wgs, stream);
+}
+
 template <int D>
 hipError_t launch_dim(const PrefixParams& p, bool is_bf16, bool wave_per_head, int own_wgs, hipStream_t stream) {
-    // pages of fewer than 32 tokens: own's form that looks up the page of every row
-    const bool small = p.own.block_table != nullptr && p.own.page_shift < 5;
-    if (is_bf16) {
-        if (wave_per_head)
-            return small ? launch_form<bf16_tag, D, true, 2>(p, own_wgs, stream) : launch_form<bf16_tag, D, true, 0>(p, own_wgs, stream);
-        return small ? launch_form<bf16_tag, D, false, 2>(p, own_wgs, stream) : launch_form<bf16_tag, D, false, 0>(p, own_wgs, stream);
-    }
-    if (wave_per_head)
-        return small ? launch_form<f16_tag, D, true, 2>(p, own_wgs, stream) : launch_form<f16_tag, D, true, 0>(p, own_wgs, stream);
-    return small ? launch_form<f16_tag, D, false, 2>(p, own_wgs, stream) : launch_form<f16_tag, D, false, 0>(p, own_wgs, stream);
+    if (is_bf16)
+        return wave_per_head ? launch_pages<bf16_tag, D, true>(p, own_wgs, stream) : launch_pages<bf16_tag, D, false>(p, own_wgs, stream);
+    return wave_per_head ? launch_pages<f16_tag, D, true>(p, own_wgs, stream) : launch_pages<f16_tag, D, false>(p, own_wgs, stream);
 }
 
 }  // namespace prefix

@@ -92,12 +92,17 @@ def test_prefix_layout_refusals():
 
 
 def test_prefix_workspace_covers_both_parts():
-    """Partials of the prefix and of the own tokens, (dim + 2) floats for every row and split."""
+    """Partials of the prefix and of the own tokens, (dim + 2) floats for every row and split; hints move the plan, and the size
+    that belongs to it is what the call asks for."""
     lib = _lib.load()
     for prefix, own, batch, hq, hk, d in [(1, 0, 1, 8, 8, 64), (4096, 1024, 64, 32, 8, 128), (8192, 128, 33, 32, 1, 256)]:
-        n = lib.da_workspace_bytes_shared_prefix(prefix, own, batch, hq, hk, d, d, 0, 0)
-        assert n >= batch * hq * (d + 2) * 4 * (2 if own else 1) and n % (batch * hq * (d + 2) * 4) == 0
-        assert n == lib.da_workspace_bytes_shared_prefix(prefix, prefix + own, batch, hq, hk, d, d, 0, 16)
+        row = batch * hq * (d + 2) * 4
+        for total in (0, 1, own * batch // 2, own * batch, 1 << 40):
+            packed = lib.da_workspace_bytes_shared_prefix(prefix, own, batch, hq, hk, d, d, total, 0)
+            paged = lib.da_workspace_bytes_shared_prefix(prefix, prefix + own, batch, hq, hk, d, d,
+                                                         total and total + prefix * batch, 16)
+            for n in (packed, paged):
+                assert row * (2 if own else 1) <= n <= row * 128
     assert lib.da_workspace_bytes_shared_prefix(64, 64, 2, 8, 3, 128, 128, 0, 0) == 0
     assert lib.da_workspace_bytes_shared_prefix(64, 64, 2, 8, 4, 576, 512, 0, 0) == 0
     # without a prefix it is the plain call's
