@@ -29,7 +29,6 @@ namespace prefix {
 // sixteen consecutive rows at one chunk (K), and four rows at four consecutive chunks (V), fall into different banks.
 // (d = 96: twelve chunks and four empty ones, so that a load instruction fills whole rows here too.)
 constexpr int kTok = 32;
-constexpr int kEarlyExp = 10;  // exponentials of a tile taken beside the next one's score products
 template <int D>
 constexpr int pitch() {
     return D == 96 ? 256 : D * 2;
@@ -42,6 +41,11 @@ __device__ __forceinline__ int swizzle(int r) {
         return mla::swz_a(r);
 }
 
+// At most N LDS reads outstanding (the other counters untouched).
+template <int N>
+__device__ __forceinline__ void wait_lds() {
+    __builtin_amdgcn_s_waitcnt(0xC07F | (N < 15 ? N : 15) << 8);
+}
 __device__ __forceinline__ auto join(s16x4_t lo, s16x4_t hi) { return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 template <int D>
@@ -134,6 +138,8 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
     };
     constexpr std::true_type kEnd{};
     constexpr std::false_type kInner{};
+    // (PGM 0, packed rows: the addresses of the tiles fetched last)
+    const uint8_t *k_next = kbase + (int64_t)(c0 + 2 * kTok) * row_bytes, *v_next = vbase + (int64_t)(c0 + kTok) * row_bytes;
     load_k(0, 0, kEnd);
     load_v(0, 0, kEnd);
     load_k(1, 1, kEnd);
@@ -173,7 +179,7 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int r = h * 4 + ((lane >> 2) & 3) + 8 * j, c = ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-            v_at[cb][j] = r * PITCH + ((cb * 4 + (c >> 3)) ^ swizzle<D>(r)) * 16 + (c & 4) * 2;
+            v_at[cb][j] = 3 * TILE + r * PITCH + ((cb * 4 + (c >> 3)) ^ swizzle<D>(r)) * 16 + (c & 4) * 2;
         }
 
     // The score tile of 32 tokens: element i is token 8 (i / 4) + 4 h + i % 4 of the tile, row n.
@@ -194,9 +200,10 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         return mx;
     };
     // ALiBi and the mask of tokens past the end, the running maximum, and (rarely) the rescaling it asks for; mx: max_of(s)
-    auto settle_max = [&](int u, float mx) __attribute__((always_inline)) {
-        const int tok0 = c0 + u * kTok;
-        if (w.is_alibi || tok0 + kTok > c1) {
+    const int plain_tiles = w.is_alibi ? 0 : (c1 - c0) / kTok;  // tiles before the first that needs either
+    auto settle_max = [&](int u, float mx, auto first_c) __attribute__((always_inline)) {
+        if (u >= plain_tiles) {
+            const int tok0 = c0 + u * kTok;
             const float at = (float)(tok0 + 4 * h - end);  // (whole numbers below 2^24: exact)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -208,6 +215,10 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             mx = max_of(s);
         }
         mx = max_xor32(mx) * mul;
+        if constexpr (decltype(first_c)::value) {  // (nothing to rescale yet)
+            m = mx > kNegBig ? mx : kNegBig;
+            return;
+        }
         const bool up = mx > m + kLazy;
         if (__any(up)) {
             const float mn = up ? mx : m;
@@ -231,8 +242,22 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         // K(u) and V(u - 1), whose buffers are filled next, are done
         if (u + 4 < nu) {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
-            load_k(u + 3, buf, kInner);
-            load_v(u + 2, prev, kInner);
+            if constexpr (PGM == 0) {
+                if (p.table == nullptr) {
+                    k_next += kTok * row_bytes;
+                    v_next += kTok * row_bytes;
+                } else {
+                    k_next = kbase + row_at(c0 + (u + 3) * kTok, w.k_page);
+                    v_next = vbase + row_at(c0 + (u + 2) * kTok, w.v_page);
+                }
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) dma16(k_next, off[i], lds0 + buf * TILE + i * 1024);
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) dma16(v_next, off[i], lds0 + (3 + prev) * TILE + i * 1024);
+            } else {
+                load_k(u + 3, buf, kInner);
+                load_v(u + 2, prev, kInner);
+            }
         } else {
             if (u + 2 < nu)
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
@@ -241,12 +266,15 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             load_k(u + 3, buf, kEnd);
             load_v(u + 2, prev, kEnd);
         }
-        // From here to the maximum the order of issue is the source's: one matrix instruction occupies its unit for 32
-        // cycles, in whose shadow go an exponential or two (16 cycles each) and the LDS reads of what comes later.
+        // From here to the maximum the order of issue is the source's: a matrix instruction occupies its unit for 32 cycles, in
+        // whose shadow go an exponential or two (16 cycles each) and the LDS reads of what comes later.  A wave issues an
+        // instruction every five cycles at best and is often alone on its SIMD, so their number counts: one wait serves
+        // several fragments, and a result of the exponential unit is not used by the next instruction, which would need a
+        // wait state.
         vec8 kf[KS];
         k_fragments(next, kf);  // (past the last tile: of whatever lies there, not used)
         typedef __attribute__((address_space(3))) s16x4_t* lds_s4;
-        uint8_t* const vt = smem + (3 + buf) * TILE;
+        uint8_t* const vt = smem + buf * TILE;  // (v_at counts the K buffers: the rest fits the instruction's offset)
         s16x4_t vf[2][CB][2];
         auto read_v = [&](int i) __attribute__((always_inline)) {  // i-th of the 4 CB reads
             const int kk = i / (2 * CB), cb = i / 2 % CB, j = i % 2;
@@ -255,47 +283,70 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         float e[16];
         uint32_t pw[8];
         constexpr uint32_t kOnes = std::is_same<Tag, f16_tag>::value ? 0x3C003C00u : 0x3F803F80u;
-        auto exponential = [&](int i) __attribute__((always_inline)) {
-            e[i] = fast_exp2(__builtin_fmaf(s[i], mul, -m));
-            if (i & 1) pw[i / 2] = EL::pack2(e[i - 1], e[i]);
+        auto exponential = [&](int i) __attribute__((always_inline)) { e[i] = fast_exp2(__builtin_fmaf(s[i], mul, -m)); };
+        auto pack = [&](int j) __attribute__((always_inline)) { pw[j] = EL::pack2(e[2 * j], e[2 * j + 1]); };
+        // Exponentials 0 .. kPre - 1 go out while the first K fragments are on their way, up to kEarly beside the score
+        // products, the rest beside the first value products; a pair is packed a slot after its second one.
+        constexpr int kPre = 4, kEarly = 12;
+        auto exps = [](int slot, int slots, int from, int to) { return from + (to - from) * slot / slots; };
+        auto packs = [&](int from, int to) __attribute__((always_inline)) {  // pairs of exponentials [from, to)
+#pragma unroll
+            for (int j = from / 2; j < to / 2; ++j) pack(j);
         };
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kPre; ++i) exponential(i);
+        __builtin_amdgcn_sched_barrier(0);
+        wait_lds<KS / 2>();
         __builtin_amdgcn_sched_barrier(0);
         f32x16 s_next;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s_next[i] = 0.0f;
         static_for<0, KS>([&](auto ks_c) __attribute__((always_inline)) {
             constexpr int ks = decltype(ks_c)::value;
+            if constexpr (ks == KS / 2) {  // the other half of the K fragments: only V reads have gone out since
+                wait_lds<4 * CB * (KS / 2) / KS>();
+                __builtin_amdgcn_sched_barrier(0);
+            }
             s_next = MM::mma(kf[ks], q[ks], s_next);
-            constexpr int e0 = kEarlyExp * ks / KS, e1 = kEarlyExp * (ks + 1) / KS;
 #pragma unroll
-            for (int i = e0; i < e1; ++i) exponential(i);
+            for (int i = exps(ks, KS, kPre, kEarly); i < exps(ks + 1, KS, kPre, kEarly); ++i) exponential(i);
 #pragma unroll
             for (int i = 4 * CB * ks / KS; i < 4 * CB * (ks + 1) / KS; ++i) read_v(i);
+            packs(ks == 0 ? 0 : exps(ks - 1, KS, kPre, kEarly), exps(ks, KS, kPre, kEarly));
             __builtin_amdgcn_sched_barrier(0);
         });
+        wait_lds<2 * CB>();  // V of the first sixteen tokens
+        __builtin_amdgcn_sched_barrier(0);
         static_for<0, CB>([&](auto cb_c) __attribute__((always_inline)) {
             constexpr int cb = decltype(cb_c)::value;
             const vec8 pf = __builtin_bit_cast(vec8, make_uint4(pw[0], pw[1], pw[2], pw[3]));
             acc[cb] = MM::mma(__builtin_bit_cast(vec8, join(vf[0][cb][0], vf[0][cb][1])), pf, acc[cb]);
-            constexpr int n_exp = 16 - kEarlyExp;
 #pragma unroll
-            for (int i = kEarlyExp + n_exp * cb / CB; i < kEarlyExp + n_exp * (cb + 1) / CB; ++i) exponential(i);
+            for (int i = exps(cb, CB, kEarly, 16); i < exps(cb + 1, CB, kEarly, 16); ++i) exponential(i);
+            // (the denominator sums the probabilities as the second product sees them)
+#pragma unroll
+            for (int j = 4 * cb / CB; j < 4 * (cb + 1) / CB; ++j) l = EL::dot2(pw[j], kOnes, l);
+            packs(cb == 0 ? exps(KS - 1, KS, kPre, kEarly) : exps(cb - 1, CB, kEarly, 16), exps(cb, CB, kEarly, 16));
             __builtin_amdgcn_sched_barrier(0);
         });
-        float mx = s_next[0];
+        packs(exps(CB - 1, CB, kEarly, 16), 16);
+        wait_lds<0>();
+        __builtin_amdgcn_sched_barrier(0);
+        float mx = -INFINITY;
         static_for<0, CB>([&](auto cb_c) __attribute__((always_inline)) {
             constexpr int cb = decltype(cb_c)::value;
             const vec8 pf = __builtin_bit_cast(vec8, make_uint4(pw[4], pw[5], pw[6], pw[7]));
             acc[cb] = MM::mma(__builtin_bit_cast(vec8, join(vf[1][cb][0], vf[1][cb][1])), pf, acc[cb]);
-            // (the denominator sums the probabilities as the second product sees them)
 #pragma unroll
-            for (int j = 8 * cb / CB; j < 8 * (cb + 1) / CB; ++j) l = EL::dot2(pw[j], kOnes, l);
+            for (int j = 4 + 4 * cb / CB; j < 4 + 4 * (cb + 1) / CB; ++j) l = EL::dot2(pw[j], kOnes, l);
 #pragma unroll
-            for (int i = 16 * cb / CB; i < 16 * (cb + 1) / CB; ++i) mx = fmaxf(mx, s_next[i]);
+            for (int j = 8 * cb / CB; j < 8 * (cb + 1) / CB; ++j) mx = fmaxf(fmaxf(mx, s_next[2 * j]), s_next[2 * j + 1]);
+            asm volatile("" : "+v"(mx));  // (here, not where it is used)
             __builtin_amdgcn_sched_barrier(0);
         });
         s = s_next;
-        if (u + 1 < nu) settle_max(u + 1, mx);
+        if (u + 1 < nu) settle_max(u + 1, mx, std::false_type{});
     };
 
     // the first tile's scores
@@ -308,7 +359,7 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         k_fragments(0, kf);
         s = scores(kf);
     }
-    settle_max(0, max_of(s));
+    settle_max(0, max_of(s), std::true_type{});
     for (int u = 0; u < nu; u += 3) {
         step(u, std::integral_constant<int, 0>{});
         if (u + 1 < nu) step(u + 1, std::integral_constant<int, 1>{});
@@ -316,16 +367,40 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
     }
 
     l += __shfl_xor(l, 32);
-    if (!live) return;
-    const size_t part = (size_t)split * w.batch * w.head_q + (size_t)b * w.head_q + hq;
-    float* const out = p.ws_o + part * D + h * 4;
+    // The partials leave through LDS, whole runs of a row at a time (the lanes hold 16 bytes of 32 rows each), and with stores
+    // that do not stay in the L2: the merge runs anywhere, and what the L2 holds is written out at the kernel's end, all of it at
+    // once (64 sequences behind 4096 tokens, 32/8 heads d 128: 51.8 -> 49.3 us).
+    const int row_id = b * w.head_q + hq;
+    const size_t part0 = (size_t)split * w.batch * w.head_q;
+    if (live && h == 0) *reinterpret_cast<float2*>(p.ws_ml + (part0 + row_id) * 2) = make_float2(m, l);
+    constexpr int GB = D == 64 ? 1 : 2;  // blocks of 32 columns at a time
+    constexpr int OPITCH = GB * 128 + 16, LPR = GB * 8, RPI = 64 / LPR;  // lanes per row, rows of a store instruction
+    static_assert(4 * 32 * OPITCH <= (int)prefix_lds_bytes<D>(), "fits the tile buffers");
+    int id[32 / RPI];  // the rows that this lane stores pieces of
 #pragma unroll
-    for (int cb = 0; cb < CB; ++cb)
+    for (int i = 0; i < 32 / RPI; ++i) id[i] = __shfl(row_id, i * RPI + lane / LPR);
+    const int rows_here = p.rows - (row0 + wave * 32);
+    __syncthreads();  // (the tiles are dead)
+    if (rows_here <= 0) return;
+    uint8_t* const mine = smem + wave * (32 * OPITCH);
+    static_for<0, (CB + GB - 1) / GB>([&](auto g_c) __attribute__((always_inline)) {
+        constexpr int cb0 = decltype(g_c)::value * GB, NB = CB - cb0 < GB ? CB - cb0 : GB;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f32x4*>(out + cb * 32 + i * 8) =
-                f32x4{acc[cb][4 * i], acc[cb][4 * i + 1], acc[cb][4 * i + 2], acc[cb][4 * i + 3]};
-    if (h == 0) *reinterpret_cast<float2*>(p.ws_ml + part * 2) = make_float2(m, l);
+        for (int cb = 0; cb < NB; ++cb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(mine + n * OPITCH + cb * 128 + i * 32 + h * 16) =
+                    f32x4{acc[cb0 + cb][4 * i], acc[cb0 + cb][4 * i + 1], acc[cb0 + cb][4 * i + 2], acc[cb0 + cb][4 * i + 3]};
+        const int piece = lane % LPR;
+        float* const out = p.ws_o + part0 * D + cb0 * 32 + piece * 4;
+#pragma unroll
+        for (int i = 0; i < 32 / RPI; ++i) {
+            if (i * RPI >= rows_here) break;
+            const int r = i * RPI + lane / LPR;
+            const f32x4 x = *reinterpret_cast<const f32x4*>(mine + r * OPITCH + piece * 16);
+            if (r < rows_here && (NB == GB || piece < NB * 8)) __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(out + (size_t)id[i] * D));
+        }
+    });
 }
 
 // Own tokens of sequence b (paged sequences count the prefix in their lengths).

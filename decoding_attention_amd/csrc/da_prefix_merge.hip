@@ -25,6 +25,16 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(const PrefixParams p)
     float mm = kNegBig, den = 0.0f;
     f32x4 num = {0.0f, 0.0f, 0.0f, 0.0f};
     if (live) {
+        // Four partials at a time.  The first four are asked for before the sequence's length is known, as far as they are the
+        // prefix's: their trip to memory runs beside the length's.
+        float2 e[4];
+        f32x4 x[4];
+        auto fetch = [&](const float* ml, const float* o, size_t part, int u) __attribute__((always_inline)) {
+            e[u] = reinterpret_cast<const float2*>(ml)[part];
+            x[u] = reinterpret_cast<const f32x4*>(o)[part * C4 + c4];
+        };
+#pragma unroll
+        for (int u = 0; u < 4; ++u) fetch(p.ws_ml, p.ws_o, (size_t)min(g + u * G, p.splits - 1) * rows + row, u);
         const int b = row / w.head_q;
         int own = p.table ? w.seq_lens[b] - p.prefix_len : w.cu_seq_k[b + 1] - w.cu_seq_k[b];
         np = own < 0 ? 0 : p.splits;  // (a row of the batch without a sequence)
@@ -42,15 +52,13 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(const PrefixParams p)
         }
         const int count = np + ns;
         for (int j0 = g; j0 < count; j0 += 4 * G) {
-            float2 e[4];
-            f32x4 x[4];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
                 const int j = min(j0 + u * G, count - 1);
-                const bool pre = j < np;
-                const size_t part = pre ? (size_t)j * rows + row : own0 + (size_t)(j - np) * stride;
-                e[u] = reinterpret_cast<const float2*>(pre ? p.ws_ml : w.ws_ml)[part];
-                x[u] = reinterpret_cast<const f32x4*>(pre ? p.ws_o : w.ws_o)[part * C4 + c4];
+                if (j >= np)
+                    fetch(w.ws_ml, w.ws_o, own0 + (size_t)(j - np) * stride, u);
+                else if (j0 != g)
+                    fetch(p.ws_ml, p.ws_o, (size_t)j * rows + row, u);
             }
             float mn = mm;
 #pragma unroll
