@@ -1403,7 +1403,7 @@ struct PrefixPlan {
     int row_tiles = 0, splits = 0, chunk = 0, prefix_wgs = 0;
     int groups = 0, own_splits = 0, own_chunk = 1, own_groups = 0;
     int flat_wgs = 0, flat_step = 1, flat_min = 1, flat_unit = 1;  // balanced own part (see Plan)
-    bool scan = false;
+    bool scan = false, spread = false;
     long long own_wgs = 0;
     size_t prefix_parts = 0, own_parts = 0;  // partial rows of either part
     size_t flat_cu_bytes = 0, ws_bytes = 0;
@@ -1454,23 +1454,29 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
 
     // Splits of the prefix: the least of (the longer of both parts' times) + (the partials' way out and back).  A work-group
     // takes 10 us and about 0.0052 us per (tile, column); one runs on a CU beside an own one (d = 256: alone), two where the own
-    // tokens are few; the (KV head, split) pairs are dealt out over the eight XCDs.
+    // tokens are few.  The row tiles of a (KV head, split) pair are kept on one XCD unless dealing them out over all eight is
+    // faster with the K/V read into every L2 (64/2 heads d 128, 82 sequences behind 5120 tokens: 21 row tiles a pair, 48 -> 38 us).
     pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
     const double own_us = 4.0 * (double)own_total * (double)head_k * (double)dim / 5.0e6 + (own_max > 0 ? 6.0 : 0.0);
+    const double kv_us = 4.0 * (double)prefix_len * (double)head_k * (double)dim / 5.0e6;
     double best = 0.0;
     long long best_s = 1;
     const long long most = std::min<long long>(((long long)prefix_len + 63) / 64, 64);
     for (long long s = 1; s <= most; ++s) {
         const long long tiles = ((long long)prefix_len + 32 * s - 1) / (32 * s);
-        const long long per_xcd = ((long long)head_k * s + 7) / 8 * pl.row_tiles;
         const double part_us = 2.0 * 4.0 * (double)s * (double)batch * (double)head_q * (double)(dim + 2) / 4.0e6;
-        for (int pair = 0; pair < (dim <= 128 ? 2 : 1); ++pair) {
+        for (int form = 0; form < 4; ++form) {
+            const int pair = form & 1, spread = form >> 1;
+            if (pair && dim > 128) continue;
+            const long long per_xcd = spread ? ((long long)head_k * s * pl.row_tiles + 7) / 8 : ((long long)head_k * s + 7) / 8 * pl.row_tiles;
             const double step = 0.0052 * (double)dim * (pair ? 1.4 : 1.0);
-            const double us = 10.0 + (double)((per_xcd + 32 * (pair + 1) - 1) / (32 * (pair + 1))) * (double)tiles * step;
+            const double us = 10.0 + (spread ? 8.0 * kv_us / 4.0 : kv_us) / 2.0 +
+                              (double)((per_xcd + 32 * (pair + 1) - 1) / (32 * (pair + 1))) * (double)tiles * step;
             const double cost = (pair ? us + own_us : std::max(us, own_us)) + part_us;
             if (best == 0.0 || cost < best) {
                 best = cost;
                 best_s = s;
+                pl.spread = spread != 0;
             }
         }
     }
@@ -1479,7 +1485,8 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
     chunk = (chunk + 31) / 32 * 32;
     pl.chunk = (int)chunk;
     pl.splits = (int)(((long long)prefix_len + chunk - 1) / chunk);
-    pl.prefix_wgs = (int)(((long long)head_k * pl.splits + 7) / 8 * 8 * pl.row_tiles);
+    pl.prefix_wgs = (int)(pl.spread ? ((long long)head_k * pl.splits * pl.row_tiles + 7) / 8 * 8
+                                    : ((long long)head_k * pl.splits + 7) / 8 * 8 * pl.row_tiles);
     pl.prefix_parts = (size_t)pl.splits * batch * head_q;
     pl.ws_bytes = (pl.prefix_parts + pl.own_parts) * (dim + 2) * sizeof(float) + pl.flat_cu_bytes;
     return pl;
@@ -1560,6 +1567,7 @@ int run_shared_prefix(const void* q, const void* pk, const void* pv, const int32
     p.splits = pl.splits;
     p.chunk = pl.chunk;
     p.prefix_wgs = pl.prefix_wgs;
+    p.spread = pl.spread ? 1 : 0;
     p.own_groups = pl.own_groups;
     w.q = q;
     w.k = k;

@@ -16,7 +16,8 @@ struct PrefixParams {
     int prefix_len;
     int rows, row_tiles;          // query rows per KV head (batch * ratio), in tiles of kPrefixRows
     int splits, chunk;            // prefix splits and tokens per split (a multiple of the tile)
-    int prefix_wgs;               // work-groups in front of own's: 8 * ceil(head_k * splits / 8) * row_tiles
+    int prefix_wgs;               // work-groups in front of own's, a multiple of 8 (see prefix_kernel)
+    int spread;                   // row tiles dealt out over all XCDs, not grouped by (KV head, split)
     int own_groups;               // own's work-groups per segment: (head_k or head_k / 4) * own.groups
     int scan;                     // balanced own part over pages: the kernel adds the lengths up itself (flat_cu is written)
     int32_t* flat_out;            // [batch + 1] (scan)

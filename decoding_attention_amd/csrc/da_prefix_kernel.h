@@ -81,19 +81,20 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
     const int c0 = split * p.chunk, c1 = min(p.prefix_len, c0 + p.chunk);
     const int last = c1 - 1, nu = (c1 - c0 + kTok - 1) / kTok;
 
-    // Tile loads: load i of a wave fills RPL rows, 16 bytes a lane, from a wave-uniform address and a per-lane offset.  PGM 0:
-    // the tile lies in one page (packed rows, or pages of 32 tokens and more); PGM 2: every load in one (pages of RPL tokens
-    // and more), or a look-up per lane (smaller ones).  Tokens past the split's end repeat its last one and are masked.
+    // Tile loads: a wave fills rows 8 w .. 8 w + 7 of every tile, RPL rows an instruction, 16 bytes a lane, from the address of
+    // its first row (one page look-up: its rows lie in one page of 8 tokens and more) and per-lane offsets.  Tokens past the
+    // split's end repeat its last one and are masked.
     const int lrow = lane / SLOTS, slot = lane % SLOTS;
     const uint32_t row_bytes = (uint32_t)w.k_row * 2;
+    const int tile_last = c0 + (nu - 1) * kTok, first_last = min(tile_last + wave * 8, last);
     uint32_t off[LOADS], off_end[LOADS];  // of any tile, and of the last one
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
-        const int r = (wave * LOADS + i) * RPL + lrow;
+        const int r = wave * 8 + i * RPL + lrow;
         const int c = slot ^ swizzle<D>(r);
         const uint32_t col = (uint32_t)(c < CPR ? c : c - 8) * 16;  // (an empty chunk: any other one of the row)
-        off[i] = (uint32_t)r * row_bytes + col;
-        off_end[i] = (uint32_t)min(r, last - (c0 + (nu - 1) * kTok)) * row_bytes + col;
+        off[i] = (uint32_t)(i * RPL + lrow) * row_bytes + col;
+        off_end[i] = (uint32_t)(min(tile_last + r, last) - first_last) * row_bytes + col;
     }
     const uint8_t* const kbase = reinterpret_cast<const uint8_t*>(p.k) + (size_t)hk * D * 2;
     const uint8_t* const vbase = reinterpret_cast<const uint8_t*>(p.v) + (size_t)hk * D * 2;
@@ -106,45 +107,40 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         if (p.table == nullptr) return (int64_t)j * w.k_row * 2;
         return ((int64_t)table[j >> w.page_shift] * page_stride + (int64_t)(j & page_mask) * w.k_row) * 2;
     };
-    // END: the tile may be the last one (or lie behind it)
-    auto load = [&](const uint8_t* base, int64_t page_stride, int u, uint32_t to, auto end_c) __attribute__((always_inline)) {
-        constexpr bool END = decltype(end_c)::value;
-        if (END && u >= nu) return;
+    auto dma_rows = [&](const uint8_t* at, const uint32_t(&o)[LOADS], uint32_t to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) dma16(at, o[i], lds0 + to + i * 1024);
+    };
+    // any tile, the last one and those behind it (which are not fetched) included
+    auto load = [&](const uint8_t* base, int64_t page_stride, int u, uint32_t to) __attribute__((always_inline)) {
+        if (u >= nu) return;
         const int tok0 = c0 + u * kTok;
-        if constexpr (PGM == 0) {
-            const uint8_t* const at = base + row_at(tok0, page_stride);
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) dma16(at, END && u == nu - 1 ? off_end[i] : off[i], lds0 + to + i * 1024);
-        } else if (page_mask + 1 >= RPL) {
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int r = (wave * LOADS + i) * RPL, j = END ? min(tok0 + r, last) : tok0 + r;
-                const uint32_t from = (uint32_t)(j - tok0) * row_bytes;
-                dma16(base + row_at(j, page_stride), (END && u == nu - 1 ? off_end[i] : off[i]) - from, lds0 + to + i * 1024);
-            }
-        } else {
+        if (PGM != 2 || page_mask >= 7) {
+            const uint8_t* const at = base + row_at(min(tok0 + wave * 8, last), page_stride);
+            if (u == nu - 1)
+                dma_rows(at, off_end, to);
+            else
+                dma_rows(at, off, to);
+        } else {  // smaller pages: a look-up per lane
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
-                const int r = (wave * LOADS + i) * RPL + lrow, j = min(tok0 + r, last);
+                const int j = min(tok0 + wave * 8 + i * RPL + lrow, last);
                 const int64_t at = (int64_t)p.table[j >> w.page_shift] * page_stride + (int64_t)(j & page_mask) * w.k_row;
-                const uint32_t col = off[i] - (uint32_t)r * row_bytes;
+                const uint32_t col = off[i] - (uint32_t)(i * RPL + lrow) * row_bytes;
                 mla::lds_dma16_v(base + at * 2 + col, lds0 + to + i * 1024);
             }
         }
     };
-    auto load_k = [&](int u, int buf, auto end_c) __attribute__((always_inline)) { load(kbase, w.k_page, u, buf * TILE, end_c); };
-    auto load_v = [&](int u, int buf, auto end_c) __attribute__((always_inline)) {
-        load(vbase, w.v_page, u, (3 + buf) * TILE, end_c);
-    };
-    constexpr std::true_type kEnd{};
-    constexpr std::false_type kInner{};
-    // (PGM 0, packed rows: the addresses of the tiles fetched last)
-    const uint8_t *k_next = kbase + (int64_t)(c0 + 2 * kTok) * row_bytes, *v_next = vbase + (int64_t)(c0 + kTok) * row_bytes;
-    load_k(0, 0, kEnd);
-    load_v(0, 0, kEnd);
-    load_k(1, 1, kEnd);
-    load_v(1, 1, kEnd);
-    load_k(2, 2, kEnd);
+    auto load_k = [&](int u, int buf) __attribute__((always_inline)) { load(kbase, w.k_page, u, buf * TILE); };
+    auto load_v = [&](int u, int buf) __attribute__((always_inline)) { load(vbase, w.v_page, u, (3 + buf) * TILE); };
+    // (packed rows: this wave's addresses in the tiles fetched last)
+    const uint8_t* k_next = kbase + (int64_t)(c0 + 2 * kTok + wave * 8) * row_bytes;
+    const uint8_t* v_next = vbase + (int64_t)(c0 + kTok + wave * 8) * row_bytes;
+    load_k(0, 0);
+    load_v(0, 0);
+    load_k(1, 1);
+    load_v(1, 1);
+    load_k(2, 2);
 
     // this lane's query row: number `row` among the KV head's; rows past the last one repeat it and are not stored
     const int row = row0 + wave * 32 + n;
@@ -200,18 +196,24 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         return mx;
     };
     // ALiBi and the mask of tokens past the end, the running maximum, and (rarely) the rescaling it asks for; mx: max_of(s)
-    const int plain_tiles = w.is_alibi ? 0 : (c1 - c0) / kTok;  // tiles before the first that needs either
+    const int whole = (c1 - c0) / kTok, plain_tiles = w.is_alibi ? 0 : whole;  // tiles before the first that needs either
     auto settle_max = [&](int u, float mx, auto first_c) __attribute__((always_inline)) {
         if (u >= plain_tiles) {
-            const int tok0 = c0 + u * kTok;
-            const float at = (float)(tok0 + 4 * h - end);  // (whole numbers below 2^24: exact)
+            const int tok0 = c0 + u * kTok + 4 * h;
+            if (w.is_alibi) {
+                const float at = slope * (float)(tok0 - end);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int j = (i >> 2) * 8 + (i & 3);
-                const float x = s[i] * w.scale_log2 + slope * (at + (float)j);
-                s[i] = tok0 + 4 * h + j >= c1 ? -INFINITY : x;
+                for (int i = 0; i < 16; ++i) {
+                    const int j = (i >> 2) * 8 + (i & 3);
+                    s[i] = __builtin_fmaf(s[i], w.scale_log2, __builtin_fmaf(slope, (float)j, at));
+                }
+                mul = 1.0f;
             }
-            mul = 1.0f;
+            if (u >= whole) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (tok0 + (i >> 2) * 8 + (i & 3) >= c1) s[i] = -INFINITY;
+            }
             mx = max_of(s);
         }
         mx = max_xor32(mx) * mul;
@@ -242,29 +244,27 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         // K(u) and V(u - 1), whose buffers are filled next, are done
         if (u + 4 < nu) {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
-            if constexpr (PGM == 0) {
+            if (PGM != 2 || page_mask >= 7) {
                 if (p.table == nullptr) {
                     k_next += kTok * row_bytes;
                     v_next += kTok * row_bytes;
                 } else {
-                    k_next = kbase + row_at(c0 + (u + 3) * kTok, w.k_page);
-                    v_next = vbase + row_at(c0 + (u + 2) * kTok, w.v_page);
+                    k_next = kbase + row_at(c0 + (u + 3) * kTok + wave * 8, w.k_page);
+                    v_next = vbase + row_at(c0 + (u + 2) * kTok + wave * 8, w.v_page);
                 }
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i) dma16(k_next, off[i], lds0 + buf * TILE + i * 1024);
-#pragma unroll
-                for (int i = 0; i < LOADS; ++i) dma16(v_next, off[i], lds0 + (3 + prev) * TILE + i * 1024);
+                dma_rows(k_next, off, buf * TILE);
+                dma_rows(v_next, off, (3 + prev) * TILE);
             } else {
-                load_k(u + 3, buf, kInner);
-                load_v(u + 2, prev, kInner);
+                load_k(u + 3, buf);
+                load_v(u + 2, prev);
             }
         } else {
             if (u + 2 < nu)
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
             else
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            load_k(u + 3, buf, kEnd);
-            load_v(u + 2, prev, kEnd);
+            load_k(u + 3, buf);
+            load_v(u + 2, prev);
         }
         // From here to the maximum the order of issue is the source's: a matrix instruction occupies its unit for 32 cycles, in
         // whose shadow go an exponential or two (16 cycles each) and the LDS reads of what comes later.  A wave issues an
@@ -442,7 +442,8 @@ __device__ __forceinline__ void scan_lengths(const PrefixParams& p, int32_t* at)
 constexpr size_t kScanBytes = (kScanBatch + 1 + 4) * sizeof(int32_t);
 
 // Work-groups are numbered so that the row tiles of one (KV head, prefix split) run on one XCD (consecutive work-groups go
-// to the eight XCDs in turn) and share its K/V through that XCD's L2; likewise the head groups of one own-token segment.
+// to the eight XCDs in turn) and share its K/V through that XCD's L2; likewise the head groups of one own-token segment.  Where
+// that leaves XCDs idle (spread) the tiles go to all of them in turn, and every L2 gets the K/V.
 //
 // The own tokens are cut in one of two ways, as in the grouped kernel: own.flat_wgs == 0: (sequence, split of own.chunk tokens);
 // else the sequences' tokens form one line, and each of flat_wgs shares of it is one work-group's (per KV heads and group).
@@ -451,11 +452,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int id = (int)blockIdx.x;
     if (id < p.prefix_wgs) {
-        const int slot = id >> 3, rest = slot / p.row_tiles;
-        const int g = rest * 8 + (id & 7);  // (KV head, split)
+        int g, tile;  // (KV head, split), row tile
+        if (p.spread) {
+            g = id / p.row_tiles;
+            tile = id - g * p.row_tiles;
+        } else {
+            const int slot = id >> 3, rest = slot / p.row_tiles;
+            g = rest * 8 + (id & 7);
+            tile = slot - rest * p.row_tiles;
+        }
         if (g >= p.own.head_k * p.splits) return;
         const int split = g / p.own.head_k;
-        prefix_segment<Tag, D, PGM>(p, smem, g - split * p.own.head_k, (slot - rest * p.row_tiles) * kPrefixRows, split);
+        prefix_segment<Tag, D, PGM>(p, smem, g - split * p.own.head_k, tile * kPrefixRows, split);
         return;
     }
     const SweepParams& w = p.own;
