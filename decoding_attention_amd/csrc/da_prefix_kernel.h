@@ -121,11 +121,17 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
                 dma_rows(at, off_end, to);
             else
                 dma_rows(at, off, to);
-        } else {  // smaller pages: a look-up per lane
+        } else {  // smaller pages: those of the wave's eight rows, each lane picking its own
+            int32_t page[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) page[r] = table[min(tok0 + wave * 8 + r, last) >> w.page_shift];
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
                 const int j = min(tok0 + wave * 8 + i * RPL + lrow, last);
-                const int64_t at = (int64_t)p.table[j >> w.page_shift] * page_stride + (int64_t)(j & page_mask) * w.k_row;
+                int32_t mine = page[i * RPL];
+#pragma unroll
+                for (int r = 1; r < RPL; ++r) mine = lrow >= r ? page[i * RPL + r] : mine;
+                const int64_t at = (int64_t)mine * page_stride + (int64_t)(j & page_mask) * w.k_row;
                 const uint32_t col = off[i] - (uint32_t)(i * RPL + lrow) * row_bytes;
                 mla::lds_dma16_v(base + at * 2 + col, lds0 + to + i * 1024);
             }
