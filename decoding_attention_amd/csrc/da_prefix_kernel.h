@@ -554,10 +554,12 @@ hipError_t launch_form(const PrefixParams& p, int own_wgs, hipStream_t stream) {
 
 template <typename Tag, int D, bool WH>
 hipError_t launch_pages(const PrefixParams& p, int own_wgs, hipStream_t stream) {
-    // how a tile's rows are found: whole tiles in pages of 32 tokens and more (and packed rows), two runs in 16-token pages,
-    // a look-up for every row in smaller ones
+    // how the own part finds a tile's rows: whole tiles in pages of 32 tokens and more (and packed rows), two runs in 16-token
+    // pages, a look-up for every row in smaller ones.  (16-token pages, 64 sequences of 1024 behind 4096, 32/8 heads, two runs
+    // against a look-up per row: d 64 38.4 / 34.4 us, d 128 50.0 / 47.5, d 96 47.1 / 52.3, d 256 98 / 158.)
     if (p.own.block_table == nullptr || p.own.page_shift >= 5) return launch_form<Tag, D, WH, 0>(p, own_wgs, stream);
-    if (p.own.page_shift == 4) return launch_form<Tag, D, WH, 1>(p, own_wgs, stream);
+    if constexpr (D == 96 || D == 256)
+        if (p.own.page_shift == 4) return launch_form<Tag, D, WH, 1>(p, own_wgs, stream);
     return launch_form<Tag, D, WH, 2>(p, own_wgs, stream);
 }
 
