@@ -338,3 +338,135 @@ def test_a_serving_loop():
     k, v = kv_cache_read(pk, pv, table, lens, cu, int(cu[-1]), dtype=dtype)
     assert torch.equal(k.cpu(), torch.cat([torch.cat([kp, t]) for t in ks]))
     assert torch.equal(v.cpu(), torch.cat([torch.cat([vp, t]) for t in vs]))
+
+
+def some(q, kp, vp, ks, vs, alibi, rows, padded=()):
+    """The reference of a few of the batch's rows."""
+    return reference(q[rows], kp, vp, [ks[b] for b in rows], [vs[b] for b in rows], alibi, live=[b not in padded for b in rows])
+
+
+# enough own tokens for equal shares of them, whatever the sequences' lengths: none, one, many shares long
+LONG_OWN = [0, 1, 3000, 17, 128, 0, 5000, 31, 32, 33, 900, 0, 64, 2500, 1, 1, 700, 4096, 129, 0]
+
+
+@pytest.mark.parametrize("page", [0, 1, 4, 8, 16, 32, 128])
+@pytest.mark.parametrize("d,hq,hk,alibi", [(128, 32, 8, False), (64, 34, 1, True), (96, 9, 3, False), (256, 36, 2, False), (128, 7, 7, True)])
+def test_own_tokens_in_equal_shares(d, hq, hk, alibi, page):
+    """Head groups (more than sixteen rows to a KV head), a wave per head and a head per work-group; padded rows."""
+    prefix, dtype, rows = 384, torch.float16 if page == 4 else torch.bfloat16, [0, 1, 2, 5, 6, 10, 13, 19]
+    q, kp, vp, ks, vs = make(len(LONG_OWN), hq, hk, d, prefix, LONG_OWN, dtype, seed=d + page)
+    padded = (5, 10) if page else ()
+    if page:
+        pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=page, padded=padded)
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, lens, most, d, alibi,
+                                                  total_k=int(lens.sum()))
+    else:
+        k, v, cu, most = packed(ks, vs, hk, d, dtype)
+        o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, alibi)
+    assert torch.isfinite(o).all()
+    check(o[rows], some(q, kp, vp, ks, vs, alibi, rows, padded))
+
+
+@pytest.mark.parametrize("batch", [1023, 1024, 1025])
+@pytest.mark.parametrize("page", [0, 16])
+def test_around_the_largest_batch_of_equal_shares(batch, page):
+    own = [(b * 41) % 150 for b in range(batch)]
+    own[-1] = 77
+    q, kp, vp, ks, vs = make(batch, 4, 4, 64, 64, own, torch.bfloat16, seed=batch)
+    rows = [0, 1, 255, 256, 500, 767, 768, 1022, batch - 1]
+    if page:
+        pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=page, padded=(500,))
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, 64, table, lens, most, 64, False)
+    else:
+        k, v, cu, most = packed(ks, vs, 4, 64, torch.bfloat16)
+        o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 64, False)
+    assert torch.isfinite(o).all()
+    check(o[rows], some(q, kp, vp, ks, vs, False, rows, (500,) if page else ()))
+
+
+@pytest.mark.parametrize("total_k", [0, 1, 384, 10 ** 9])
+def test_hints_move_no_result_out_of_tolerance(total_k):
+    """total_k and the bound on the lengths are hints: wrong ones plan badly, and change roundings at most."""
+    prefix, rows = 384, [0, 1, 2, 6, 13, 19]
+    q, kp, vp, ks, vs = make(len(LONG_OWN), 32, 8, 128, prefix, LONG_OWN, torch.bfloat16, seed=1)
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, 16, seed=1)
+    table = torch.nn.functional.pad(table, (0, 300), value=-1)
+    for bound in (most, most + 4000):
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, lens, bound, 128, False, total_k=total_k)
+        check(o[rows], some(q, kp, vp, ks, vs, False, rows))
+    k, v, cu, most = packed(ks, vs, 8, 128, torch.bfloat16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, 3 * most, 128, False)
+    check(o[rows], some(q, kp, vp, ks, vs, False, rows))
+
+
+@pytest.mark.parametrize("page", [0, 1, 16, 64])
+def test_replays_of_equal_shares_with_other_lengths(page):
+    """The shares follow the lengths on the device: shorter sequences, empty ones, and none at all under the captured plan."""
+    prefix, d = 256, 128
+    q, kp, vp, ks, vs = make(len(LONG_OWN), 32, 8, d, prefix, LONG_OWN, torch.bfloat16, seed=20 + page)
+    dq = q.to(DEV)
+    if page:
+        pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=page)
+        run = lambda: decoding_attn_paged_shared_prefix_fwd(dq, pk, pv, ids, prefix, table, lens, most, d, False)  # noqa: E731
+    else:
+        k, v, cu, most = packed(ks, vs, 8, d, torch.bfloat16)
+        dkp, dvp = kp.to(DEV), vp.to(DEV)
+        run = lambda: decoding_attn_shared_prefix_fwd(dq, dkp, dvp, k, v, cu, most, d, False)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run()
+    torch.cuda.current_stream().wait_stream(s)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run()
+        graphs.append((graph, out))
+    g = torch.Generator().manual_seed(21)
+    for step in range(4):
+        own = [0 if step == 2 else max(0, n - step * 37) for n in LONG_OWN]
+        if page:
+            lens.copy_(torch.tensor([0 if step == 3 and b % 3 == 0 else prefix + n for b, n in enumerate(own)], dtype=torch.int32))
+        else:
+            cu.copy_(torch.tensor([0] + own).cumsum(0).to(torch.int32))
+        dq.copy_(torch.randn(q.shape, generator=g).to(q.dtype))
+        for graph, out in graphs:
+            graph.replay()
+        want = run()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert torch.equal(out, want)
+        if page:  # (the packed rows move with the lengths)
+            rows, padded = [0, 1, 2, 6, 13], [b for b in range(20) if step == 3 and b % 3 == 0]
+            cut = lambda x: [t[:n] for t, n in zip(x, own)]  # noqa: E731
+            check(want[rows], some(dq.cpu(), kp, vp, cut(ks), cut(vs), False, rows, padded))
+
+
+def test_row_tiles_over_all_chiplets():
+    """Two KV heads of 21 row tiles each, few splits: more tiles than one chiplet's share of the pairs would hold."""
+    own = [(b * 7) % 9 for b in range(82)]
+    q, kp, vp, ks, vs = make(82, 64, 2, 64, 2080, own, torch.float16, seed=22)
+    k, v, cu, most = packed(ks, vs, 2, 64, torch.float16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 64, False)
+    rows = [0, 3, 4, 40, 41, 80, 81]
+    check(o[rows], some(q, kp, vp, ks, vs, False, rows))
+
+
+@pytest.mark.parametrize("page", [2, 16, 64])
+def test_pages_past_32_bit_offsets(page):
+    """Prefix and own pages at both ends of pools of more than 2^32 elements."""
+    hk, d, prefix, own = 8, 128, 192, [0, 5, 70, 1]
+    q, kp, vp, ks, vs = make(4, 32, hk, d, prefix, own, torch.bfloat16, seed=23)
+    pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=23)
+    n = pk.shape[0]
+    pages = 4_400_000_000 // (page * hk * d)
+    far = pages - n + torch.arange(n, device=DEV)  # (every second page at the start)
+    where = torch.where(torch.arange(n, device=DEV) % 2 == 0, torch.arange(n, device=DEV), far)
+    big = [torch.empty(pages, page, hk, d, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    for pool, small in zip(big, (pk, pv)):
+        for i, w in enumerate(where.tolist()):
+            pool[w].copy_(small[i])
+    table = torch.where(table >= 0, where[table.clamp(min=0).long()], -1).to(torch.int32)
+    o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), *big, where[ids.long()].to(torch.int32), prefix, table, lens, most, d, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
