@@ -59,6 +59,25 @@ __device__ __forceinline__ void dma16(const uint8_t* base, uint32_t lane_off, ui
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(lane_off), "s"(base), "s"(to) : "memory");
 }
 
+// x *= alpha in accumulation registers.  d = 256 keeps its accumulators there, which only matrix instructions and moves reach;
+// a plain product in a branch has the compiler move all 128 of them out and back in on both ways round it, every tile.
+// (The waits: for a matrix instruction's result before the first read, and before the next one reads what is written here.)
+__device__ __forceinline__ void scale_acc(f32x16& x, float alpha) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        float a = x[i], b = x[i + 1], c = x[i + 2], d = x[i + 3], t, u;
+        asm volatile(
+            "s_nop 15\n\ts_nop 15\n\t"
+            "v_accvgpr_read_b32 %4, %0\n\tv_accvgpr_read_b32 %5, %1\n\tv_mul_f32 %4, %4, %6\n\tv_mul_f32 %5, %5, %6\n\t"
+            "v_accvgpr_write_b32 %0, %4\n\tv_accvgpr_write_b32 %1, %5\n\t"
+            "v_accvgpr_read_b32 %4, %2\n\tv_accvgpr_read_b32 %5, %3\n\tv_mul_f32 %4, %4, %6\n\tv_mul_f32 %5, %5, %6\n\t"
+            "v_accvgpr_write_b32 %2, %4\n\tv_accvgpr_write_b32 %3, %5\n\ts_nop 7"
+            : "+a"(a), "+a"(b), "+a"(c), "+a"(d), "=&v"(t), "=&v"(u)
+            : "v"(alpha));
+        x[i] = a, x[i + 1] = b, x[i + 2] = c, x[i + 3] = d;
+    }
+}
+
 template <typename Tag, int D, int PGM>
 __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* const smem, const int hk, const int row0,
                                                const int split) {
@@ -234,7 +253,12 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             m = mn;
             l *= alpha;
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) acc[cb] *= alpha;
+            for (int cb = 0; cb < CB; ++cb) {
+                if constexpr (D == 256)
+                    scale_acc(acc[cb], alpha);
+                else
+                    acc[cb] *= alpha;
+            }
         }
     };
     auto k_fragments = [&](int buf, vec8(&kf)[KS]) __attribute__((always_inline)) {

@@ -198,13 +198,14 @@ def test_flat_and_steep_scores(sharp):
     check(o, reference(q, kp, vp, ks, vs, False))
 
 
-def test_a_maximum_that_rises_all_the_way():
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_a_maximum_that_rises_all_the_way(d):
     """Keys in the order of their scores: the running maximum is raised again and again."""
-    q, kp, vp, ks, vs = make(4, 4, 1, 64, 2000, [3, 300, 0, 9], torch.float16, seed=5, sharp=0.1)
+    q, kp, vp, ks, vs = make(4, 4, 1, d, 2000, [3, 300, 0, 9], torch.float16, seed=5, sharp=0.1)
     ramp = torch.linspace(-60, 60, 2000)
     q[:, :, 0], kp[:, 0, 0] = 8.0, ramp.half()
-    k, v, cu, most = packed(ks, vs, 1, 64, torch.float16)
-    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, 64, False)
+    k, v, cu, most = packed(ks, vs, 1, d, torch.float16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
     check(o, reference(q, kp, vp, ks, vs, False))
 
 
