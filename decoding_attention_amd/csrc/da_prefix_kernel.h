@@ -78,6 +78,13 @@ __device__ __forceinline__ void scale_acc(f32x16& x, float alpha) {
     }
 }
 
+// Keeps a matrix product where the source has it (d = 256: with this many registers in use the compiler puts the score products
+// behind the value products, and all of a tile's LDS reads in front of both).
+template <int D>
+__device__ __forceinline__ void pin(f32x16& x) {
+    if constexpr (D == 256) asm volatile("" : "+a"(x));
+}
+
 template <typename Tag, int D, int PGM>
 __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* const smem, const int hk, const int row0,
                                                const int split) {
@@ -339,6 +346,7 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
                 __builtin_amdgcn_sched_barrier(0);
             }
             s_next = MM::mma(kf[ks], q[ks], s_next);
+            pin<D>(s_next);
 #pragma unroll
             for (int i = exps(ks, KS, kPre, kEarly); i < exps(ks + 1, KS, kPre, kEarly); ++i) exponential(i);
 #pragma unroll
@@ -352,6 +360,7 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             constexpr int cb = decltype(cb_c)::value;
             const vec8 pf = __builtin_bit_cast(vec8, make_uint4(pw[0], pw[1], pw[2], pw[3]));
             acc[cb] = MM::mma(__builtin_bit_cast(vec8, join(vf[0][cb][0], vf[0][cb][1])), pf, acc[cb]);
+            pin<D>(acc[cb]);
 #pragma unroll
             for (int i = exps(cb, CB, kEarly, 16); i < exps(cb + 1, CB, kEarly, 16); ++i) exponential(i);
             // (the denominator sums the probabilities as the second product sees them)
@@ -368,6 +377,7 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             constexpr int cb = decltype(cb_c)::value;
             const vec8 pf = __builtin_bit_cast(vec8, make_uint4(pw[4], pw[5], pw[6], pw[7]));
             acc[cb] = MM::mma(__builtin_bit_cast(vec8, join(vf[1][cb][0], vf[1][cb][1])), pf, acc[cb]);
+            pin<D>(acc[cb]);
 #pragma unroll
             for (int j = 4 + 4 * cb / CB; j < 4 + 4 * (cb + 1) / CB; ++j) l = EL::dot2(pw[j], kOnes, l);
 #pragma unroll
