@@ -166,13 +166,13 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
     auto load_k = [&](int u, int buf) __attribute__((always_inline)) { load(kbase, w.k_page, u, buf * TILE); };
     auto load_v = [&](int u, int buf) __attribute__((always_inline)) { load(vbase, w.v_page, u, (3 + buf) * TILE); };
     // (packed rows: this wave's addresses in the tiles fetched last)
-    const uint8_t* k_next = kbase + (int64_t)(c0 + 2 * kTok + wave * 8) * row_bytes;
+    const uint8_t* k_next = kbase + (int64_t)(c0 + 3 * kTok + wave * 8) * row_bytes;
     const uint8_t* v_next = vbase + (int64_t)(c0 + kTok + wave * 8) * row_bytes;
     load_k(0, 0);
-    load_v(0, 0);
     load_k(1, 1);
-    load_v(1, 1);
+    load_v(0, 0);
     load_k(2, 2);
+    load_v(1, 1);
 
     // this lane's query row: number `row` among the KV head's; rows past the last one repeat it and are not stored
     const int row = row0 + wave * 32 + n;
@@ -268,48 +268,49 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             }
         }
     };
-    auto k_fragments = [&](int buf, vec8(&kf)[KS]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) kf[ks] = *reinterpret_cast<const vec8*>(smem + buf * TILE + k_at[ks]);
+    vec8 kf[KS];  // K fragments of the tile whose scores come next
+    auto read_k = [&](int ks, int buf) __attribute__((always_inline)) {
+        kf[ks] = *reinterpret_cast<const vec8*>(smem + buf * TILE + k_at[ks]);
     };
 
     // One tile: the score products of the next one beside this one's exponentials, then its value products beside the
-    // next one's maximum.
+    // next one's maximum and the K fragments of the one after.
     auto step = [&](int u, auto buf_c) __attribute__((always_inline)) {
         constexpr int buf = decltype(buf_c)::value, next = (buf + 1) % 3, prev = (buf + 2) % 3;
-        // K of tile u + 1 and V of tile u have landed (this wave's share; after the barrier, everyone's), and the reads of
-        // K(u) and V(u - 1), whose buffers are filled next, are done
-        if (u + 4 < nu) {
+        // K of tile u + 2 and V of tile u have landed (this wave's share; after the barrier, everyone's), and the reads of
+        // K(u + 1) and V(u - 1), whose buffers are filled next, are done
+        if (u + 5 < nu) {
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
             if (PGM != 2 || page_mask >= 7) {
                 if (p.table == nullptr) {
                     k_next += kTok * row_bytes;
                     v_next += kTok * row_bytes;
                 } else {
-                    k_next = kbase + row_at(c0 + (u + 3) * kTok + wave * 8, w.k_page);
+                    k_next = kbase + row_at(c0 + (u + 4) * kTok + wave * 8, w.k_page);
                     v_next = vbase + row_at(c0 + (u + 2) * kTok + wave * 8, w.v_page);
                 }
-                dma_rows(k_next, off, buf * TILE);
+                dma_rows(k_next, off, next * TILE);
                 dma_rows(v_next, off, (3 + prev) * TILE);
             } else {
-                load_k(u + 3, buf);
+                load_k(u + 4, next);
                 load_v(u + 2, prev);
             }
         } else {
-            if (u + 2 < nu)
+            if (u + 3 < nu)
                 asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * LOADS) : "memory");
+            else if (u + 1 < nu)
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LOADS) : "memory");
             else
                 asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            load_k(u + 3, buf);
+            load_k(u + 4, next);
             load_v(u + 2, prev);
         }
         // From here to the maximum the order of issue is the source's: a matrix instruction occupies its unit for 32 cycles, in
         // whose shadow go an exponential or two (16 cycles each) and the LDS reads of what comes later.  A wave issues an
         // instruction every five cycles at best and is often alone on its SIMD, so their number counts: one wait serves
         // several fragments, and a result of the exponential unit is not used by the next instruction, which would need a
-        // wait state.
-        vec8 kf[KS];
-        k_fragments(next, kf);  // (past the last tile: of whatever lies there, not used)
+        // wait state.  (The K fragments are read in the step before: a step that begins with their reads begins with the latency
+        // of all four waves' at once.)
         typedef __attribute__((address_space(3))) s16x4_t* lds_s4;
         uint8_t* const vt = smem + buf * TILE;  // (v_at counts the K buffers: the rest fits the instruction's offset)
         s16x4_t vf[2][CB][2];
@@ -322,29 +323,20 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         constexpr uint32_t kOnes = std::is_same<Tag, f16_tag>::value ? 0x3C003C00u : 0x3F803F80u;
         auto exponential = [&](int i) __attribute__((always_inline)) { e[i] = fast_exp2(__builtin_fmaf(s[i], mul, -m)); };
         auto pack = [&](int j) __attribute__((always_inline)) { pw[j] = EL::pack2(e[2 * j], e[2 * j + 1]); };
-        // Exponentials 0 .. kPre - 1 go out while the first K fragments are on their way, up to kEarly beside the score
-        // products, the rest beside the first value products; a pair is packed a slot after its second one.
-        constexpr int kPre = 4, kEarly = 12;
+        // Exponentials up to kEarly go out beside the score products, the rest beside the first value products; a pair is packed
+        // a slot after its second one.
+        constexpr int kPre = 0, kEarly = 12;
         auto exps = [](int slot, int slots, int from, int to) { return from + (to - from) * slot / slots; };
         auto packs = [&](int from, int to) __attribute__((always_inline)) {  // pairs of exponentials [from, to)
 #pragma unroll
             for (int j = from / 2; j < to / 2; ++j) pack(j);
         };
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < kPre; ++i) exponential(i);
-        __builtin_amdgcn_sched_barrier(0);
-        wait_lds<KS / 2>();
-        __builtin_amdgcn_sched_barrier(0);
         f32x16 s_next;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s_next[i] = 0.0f;
         static_for<0, KS>([&](auto ks_c) __attribute__((always_inline)) {
             constexpr int ks = decltype(ks_c)::value;
-            if constexpr (ks == KS / 2) {  // the other half of the K fragments: only V reads have gone out since
-                wait_lds<4 * CB * (KS / 2) / KS>();
-                __builtin_amdgcn_sched_barrier(0);
-            }
             s_next = MM::mma(kf[ks], q[ks], s_next);
             pin<D>(s_next);
 #pragma unroll
@@ -367,10 +359,12 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
 #pragma unroll
             for (int j = 4 * cb / CB; j < 4 * (cb + 1) / CB; ++j) l = EL::dot2(pw[j], kOnes, l);
             packs(cb == 0 ? exps(KS - 1, KS, kPre, kEarly) : exps(cb - 1, CB, kEarly, 16), exps(cb, CB, kEarly, 16));
+#pragma unroll
+            for (int ks = cb; ks < KS / 2; ks += CB) read_k(ks, prev);  // (past the last tile: of whatever lies there, not used)
             __builtin_amdgcn_sched_barrier(0);
         });
         packs(exps(CB - 1, CB, kEarly, 16), 16);
-        wait_lds<0>();
+        wait_lds<KS / 2>();  // V of the other sixteen
         __builtin_amdgcn_sched_barrier(0);
         float mx = -INFINITY;
         static_for<0, CB>([&](auto cb_c) __attribute__((always_inline)) {
@@ -383,22 +377,29 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
 #pragma unroll
             for (int j = 8 * cb / CB; j < 8 * (cb + 1) / CB; ++j) mx = fmaxf(fmaxf(mx, s_next[2 * j]), s_next[2 * j + 1]);
             asm volatile("" : "+v"(mx));  // (here, not where it is used)
+#pragma unroll
+            for (int ks = KS / 2 + cb; ks < KS; ks += CB) read_k(ks, prev);
             __builtin_amdgcn_sched_barrier(0);
         });
         s = s_next;
         if (u + 1 < nu) settle_max(u + 1, mx, std::false_type{});
     };
 
-    // the first tile's scores
+    // the first tile's scores, and the K fragments of the second
     if (nu > 2)
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * LOADS) : "memory");
     else
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    {
-        vec8 kf[KS];
-        k_fragments(0, kf);
-        s = scores(kf);
-    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) read_k(ks, 0);
+    s = scores(kf);
+    if (nu > 2)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * LOADS) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    load_k(3, 0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) read_k(ks, 1);
     settle_max(0, max_of(s), std::true_type{});
     for (int u = 0; u < nu; u += 3) {
         step(u, std::integral_constant<int, 0>{});
