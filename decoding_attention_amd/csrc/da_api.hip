@@ -1419,9 +1419,59 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
     pl.wave_per_head = head_k % 4 == 0;
     pl.groups = (int)((ratio + 15) / 16);
     pl.own_groups = (int)(pl.wave_per_head ? head_k / 4 : head_k) * pl.groups;
+    // Splits of the prefix, by the expected time of both parts and of the partials' way out and back.  A prefix work-group takes
+    // 10 us and `step` per 32-token tile, 1.7 times that beside own work-groups (32/8 heads d 128, 16384 tokens: 0.61 and 1.1 us;
+    // d 64 0.48 and 0.75; d 256 0.85 alone) or beside a second one.  Up to d = 128 a CU holds one of each kind, or two; at
+    // d = 256 one.  The row tiles of a (KV head, split) pair are kept on one XCD unless dealing them out over all eight is
+    // faster with the K/V read into every L2 (64/2 heads d 128, 82 sequences behind 5120 tokens: 21 row tiles a pair, 48 -> 38 us).
+    pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
+    const double own_us = own_max > 0 ? 4.0 * (double)own_total * (double)head_k * (double)dim / 5.0e6 + 6.0 : 0.0;
+    const double kv_us = 4.0 * (double)prefix_len * (double)head_k * (double)dim / 5.0e6;
+    const double step = 0.34 + 0.0021 * (double)dim, beside = 1.7 * step;
+    const long long most = std::min<long long>(((long long)prefix_len + 63) / 64, 64);
+    const long long forced = tun().prefix_splits > 0 ? std::min<long long>(tun().prefix_splits, most) : 0;
+    double best = 0.0;
+    long long best_s = 1;
+    bool beside_prefix = false;
+    for (long long s = forced ? forced : 1; s <= (forced ? forced : most); ++s) {
+        const long long tiles = ((long long)prefix_len + 32 * s - 1) / (32 * s);
+        const double part_us = 2.0 * 4.0 * (double)s * (double)batch * (double)head_q * (double)(dim + 2) / 4.0e6;
+        if (best > 0.0 && part_us + own_us >= best) break;
+        for (int spread = 0; spread < 2; ++spread) {
+            const long long per_xcd =
+                spread ? ((long long)head_k * s * pl.row_tiles + 7) / 8 : ((long long)head_k * s + 7) / 8 * pl.row_tiles;
+            const double start = 10.0 + (spread ? 8.0 * kv_us / 4.0 : kv_us) / 2.0;
+            const double one = (double)((per_xcd + 31) / 32 * tiles), two = (double)((per_xcd + 63) / 64 * tiles);  // steps in a row
+            double us;
+            bool share_cus = false;
+            if (dim > 128) {  // own work-groups have the CUs that the prefix leaves, if they are fewer, or come behind it
+                const double left = (double)(32 - per_xcd) / 32.0, both = std::max(start + one * step, own_us * 1.25 / left);
+                us = start + one * step + own_us * 1.25;
+                share_cus = per_xcd <= 24 && both < us;
+                if (share_cus) us = both;
+            } else {
+                us = one * beside <= own_us ? one * beside : own_us + (one - own_us / beside) * step;
+                us = std::max(start + us, own_us + 0.2 * std::min(start + us, own_us));
+                us = std::min(us, start + two * beside + own_us);
+            }
+            if (best == 0.0 || us + part_us < best) {
+                best = us + part_us;
+                best_s = s;
+                beside_prefix = share_cus;
+                pl.spread = spread != 0;
+            }
+        }
+    }
+    long long chunk = ((long long)prefix_len + best_s - 1) / best_s;
+    chunk = (chunk + 31) / 32 * 32;
+    pl.chunk = (int)chunk;
+    pl.splits = (int)(((long long)prefix_len + chunk - 1) / chunk);
+    pl.prefix_wgs = (int)(pl.spread ? ((long long)head_k * pl.splits * pl.row_tiles + 7) / 8 * 8
+                                    : ((long long)head_k * pl.splits + 7) / 8 * 8 * pl.row_tiles);
     if (own_max > 0) {
         const long long trip = pl.wave_per_head ? da::kGqaTile : 4 * da::kGqaTile;
-        const long long target = tun().prefix_own_wgs * (dim == 64 ? 2 : 1), shares = std::max<long long>(1, target / pl.own_groups);
+        const long long target = dim == 64 ? 2 * tun().prefix_own_wgs : tun().prefix_own_wgs - (beside_prefix ? pl.prefix_wgs : 0);
+        const long long shares = std::max<long long>(1, target / pl.own_groups);
         // equal shares where every one gets 128 tokens and more: 256 sequences of 0 .. 1024 own tokens, 32/8 heads d 128, 102 us
         // where splits of 1024 tokens take 145
         const long long unit = page_size == 0 ? 1 : da::kGqaTile;
@@ -1438,7 +1488,10 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
             if (pl.scan) pl.flat_cu_bytes = ((batch + 1) * sizeof(int32_t) + 15) / 16 * 16;
         } else {
             const long long base = (long long)batch * pl.own_groups;
-            long long ns = std::max<long long>(1, 512 / base);
+            // (a second work-group per CU where each still has some 64 KB of K and V per head, 32/8 heads d 128: 8 sequences of
+            // 4000 own tokens 31.6 -> 27.6 us, 4 of 8000 30.8 -> 21.4; d 256, 8 of 2000, 34.5 -> 29.9; but 16 of 1000 25.8 -> 29.3)
+            long long ns = std::max<long long>(1, target / base);
+            if (target < 512 && (long long)own_max / ns * (long long)dim >= (dim > 128 ? 15000 : 30000)) ns = std::max<long long>(1, 512 / base);
             ns = std::max(ns, ((long long)own_max + 1023) / 1024);
             ns = std::min(ns, ((long long)own_max + trip - 1) / trip);
             long long oc = ((long long)own_max + ns - 1) / ns;
@@ -1451,42 +1504,6 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
             (pl.flat_wgs ? (long long)pl.flat_wgs : (long long)batch * pl.own_splits) * (pl.own_groups / pl.groups);
         pl.own_wgs = pl.groups > 1 ? (segs + 7) / 8 * 8 * pl.groups : segs;
     }
-
-    // Splits of the prefix: the least of (the longer of both parts' times) + (the partials' way out and back).  A work-group
-    // takes 10 us and about 0.0052 us per (tile, column); one runs on a CU beside an own one (d = 256: alone), two where the own
-    // tokens are few.  The row tiles of a (KV head, split) pair are kept on one XCD unless dealing them out over all eight is
-    // faster with the K/V read into every L2 (64/2 heads d 128, 82 sequences behind 5120 tokens: 21 row tiles a pair, 48 -> 38 us).
-    pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
-    const double own_us = 4.0 * (double)own_total * (double)head_k * (double)dim / 5.0e6 + (own_max > 0 ? 6.0 : 0.0);
-    const double kv_us = 4.0 * (double)prefix_len * (double)head_k * (double)dim / 5.0e6;
-    double best = 0.0;
-    long long best_s = 1;
-    const long long most = std::min<long long>(((long long)prefix_len + 63) / 64, 64);
-    for (long long s = 1; s <= most; ++s) {
-        const long long tiles = ((long long)prefix_len + 32 * s - 1) / (32 * s);
-        const double part_us = 2.0 * 4.0 * (double)s * (double)batch * (double)head_q * (double)(dim + 2) / 4.0e6;
-        for (int form = 0; form < 4; ++form) {
-            const int pair = form & 1, spread = form >> 1;
-            if (pair && dim > 128) continue;
-            const long long per_xcd = spread ? ((long long)head_k * s * pl.row_tiles + 7) / 8 : ((long long)head_k * s + 7) / 8 * pl.row_tiles;
-            const double step = 0.0052 * (double)dim * (pair ? 1.4 : 1.0);
-            const double us = 10.0 + (spread ? 8.0 * kv_us / 4.0 : kv_us) / 2.0 +
-                              (double)((per_xcd + 32 * (pair + 1) - 1) / (32 * (pair + 1))) * (double)tiles * step;
-            const double cost = (pair ? us + own_us : std::max(us, own_us)) + part_us;
-            if (best == 0.0 || cost < best) {
-                best = cost;
-                best_s = s;
-                pl.spread = spread != 0;
-            }
-        }
-    }
-    if (tun().prefix_splits > 0) best_s = std::min<long long>(tun().prefix_splits, most);
-    long long chunk = ((long long)prefix_len + best_s - 1) / best_s;
-    chunk = (chunk + 31) / 32 * 32;
-    pl.chunk = (int)chunk;
-    pl.splits = (int)(((long long)prefix_len + chunk - 1) / chunk);
-    pl.prefix_wgs = (int)(pl.spread ? ((long long)head_k * pl.splits * pl.row_tiles + 7) / 8 * 8
-                                    : ((long long)head_k * pl.splits + 7) / 8 * 8 * pl.row_tiles);
     pl.prefix_parts = (size_t)pl.splits * batch * head_q;
     pl.ws_bytes = (pl.prefix_parts + pl.own_parts) * (dim + 2) * sizeof(float) + pl.flat_cu_bytes;
     return pl;
