@@ -20,9 +20,8 @@ constexpr int kThreads = 256;
 constexpr int kUnroll = 4;        // chunks a thread holds at once
 constexpr int kMaxTokens = 128;   // most tokens of a work-group
 
-// i / d for 0 <= i < 2^16 * 2^11, d <= 2^16, by m = ceil(2^32 / d): the excess of m is below 2^-32 d, so the quotient is
-// right while i * d < 2^32 (here i < 2048 + d and the two never reach it together: a work-group holds at most
-// kThreads * kUnroll chunks, or the chunks of one token)
+// i / d by m = ceil(2^32 / d): the excess of m is below 2^-32 d, so the quotient is right while i * d < 2^32 (a work-group holds at
+// most 2 kThreads * kUnroll chunks, or the chunks of one token, of which there are 2^15 at most)
 __device__ __forceinline__ int magic_div(int i, uint32_t m) { return (int)__umulhi((uint32_t)i, m); }
 
 // Where a token's row lies in the plane's pool.
@@ -203,11 +202,12 @@ __device__ __forceinline__ float not_finite(uint4 w, float seen) {
 }
 
 // The same for ordinary values at a fourth of the instructions, sixteen integers packed into four words (int4: two).
-// t = x inv + zero is taken in double precision with one rounding, and one addition brings t + 1/2 into the low word of a double
-// as a fixed-point number, the integer in its upper bits.  t, and the definition's quotient and sum, are off by less than 2^-40
-// (|zero| < 2^20), the fixed point by half a unit of 2^-24 (int8) or 2^-28 (int4): where t + 1/2 lies more than a unit from a whole
-// number the integer is the definition's.  The others (of normal values, a lane's sixteen in 200) are settled by the quotient
-// itself.
+// One multiply-add in double precision, x inv + (zero + 1/2 + a constant of 1.5 2^28 or 1.5 2^24), leaves t + 1/2 in the low word as
+// a fixed-point number in units of 2^-24 (int8) or 2^-28 (int4), the integer in its upper bits.  It is off by a unit at most, half
+// from the sum in brackets and half from the result (inv, and the definition's quotient and sum, by less than 2^-40: |zero| < 2^20),
+// and two are added: a fraction of five units and more lies behind the whole number that the definition rounds to, and one that
+// passed the next whole number counts three at most.  The others (of normal values, a lane's sixteen in 200) are settled by the
+// quotient itself.
 template <typename Tag, int FMT, int PAIRS>
 __device__ __forceinline__ void quantise(const uint4 (&raw)[2], const uint16_t* src, float factor, int span, uint32_t (&w)[4],
                                          float2& pair) {
@@ -244,26 +244,29 @@ __device__ __forceinline__ void quantise(const uint4 (&raw)[2], const uint16_t* 
         inv = 1.0 / (double)factor;
         plain = plain && factor > 1e-30f && factor < 1e30f;
     }
-    const double s = (double)pair.x, z = (double)pair.y;
+    const double s = (double)pair.x, z = (double)pair.y, zc = z + (1.5 * 0x1p52 * kUnit + 0.5 + 2.0 * kUnit);
     const float least = factor * (QLO - 0.25f), most = factor * (QHI + 0.25f);
     uint32_t near = ~0u;
 #pragma unroll
     for (int j = 15; j >= 0; --j) {
         // (factors per head: what lies beyond the range is cut to just outside the outermost integers)
         const float c = PAIRS == 0 ? __builtin_amdgcn_fmed3f(x[j], least, most) : x[j];
-        const double u = fma((double)c, inv, z) + (1.5 * 0x1p52 * kUnit + 0.5 + kUnit);
+        const double u = fma((double)c, inv, zc);
         const uint32_t v = (uint32_t)__double_as_longlong(u);
-        near = min(near, v << BITS);  // (the fraction; one unit was added: 0, 1 and 2 are too near)
+        near = min(near, v << BITS);  // (the fraction)
         w[j / PER] = __builtin_amdgcn_alignbit(j % PER == PER - 1 ? 0u : w[j / PER], v, 32 - BITS);
     }
-    const bool sure = near >= (3u << BITS);
+    const bool sure = near >= (5u << BITS);
     if (__any(!(plain && sure))) {
         if (__any(!plain)) {
             quantise_any<Tag, FMT, PAIRS>(src, factor, span, w, pair);
         } else {
+            uint32_t again[8] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) asm volatile("" : "+v"(again[j]));  // (widened once more: x is not kept for this)
 #pragma unroll
             for (int j = 15; j >= 0; --j) {
-                const double y = quotient((double)x[j], s, inv);
+                const double y = quotient((double)(j & 1 ? Elem<Tag>::hi(again[j >> 1]) : Elem<Tag>::lo(again[j >> 1])), s, inv);
                 const uint32_t n = (uint32_t)to_int<QLO, QHI>(PAIRS == 0 ? y : y + z) << (32 - BITS);
                 w[j / PER] = __builtin_amdgcn_alignbit(j % PER == PER - 1 ? 0u : w[j / PER], n, 32 - BITS);
             }
@@ -479,11 +482,16 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const KvCacheParams p
     }
 }
 
-// Tokens per work-group: a thread holds up to kUnroll chunks, fewer while that leaves CUs without a work-group.
-int tokens_per_block(const KvCacheParams& p, int planes, int elems) {
+// Tokens per work-group: a thread holds up to kUnroll chunks, fewer while that leaves CUs without a work-group.  Large calls
+// take two turns, for the rows' look-up is three trips to memory one after the other: int8 with a pair per 64, 26 000 tokens of
+// 8 heads d 128, 47.2 -> 39.2 us with half the work-groups; a read looks up less beside more bytes, int4 per 64, 114 000 tokens, 138 ->
+// 132 us, and 29.5 -> 30.0 at a quarter of that.
+int tokens_per_block(const KvCacheParams& p, bool read, int planes, int elems) {
     const int chunks = p.head_k * (p.plane[0].dim >> 3);  // (of eight elements: kUnroll of them to a thread)
     int tpb = kThreads * kUnroll / chunks;
-    while (tpb > 1 && tpb * chunks > kThreads * elems / 8 && (p.tokens + tpb - 1) / tpb * planes < 512) tpb >>= 1;
+    const auto groups = [&](int t) { return (p.tokens + t - 1) / t * planes; };
+    if (tpb > 0 && 2 * tpb <= kMaxTokens && groups(2 * tpb) >= (read ? 8192 : 1024)) return 2 * tpb;
+    while (tpb > 1 && tpb * chunks > kThreads * elems / 8 && groups(tpb) < 512) tpb >>= 1;
     return tpb < 1 ? 1 : (tpb > kMaxTokens ? kMaxTokens : tpb);
 }
 
@@ -500,7 +508,7 @@ hipError_t launch_form(const KvCacheParams& p, int planes, hipStream_t stream) {
 template <bool READ, typename Tag>
 hipError_t launch_tag(KvCacheParams p, int fmt, int pairs, int planes, hipStream_t stream) {
     const int elems = READ || fmt == 0 ? 8 : 16;  // append_chunk()
-    p.tokens_per_block = tokens_per_block(p, planes, elems);
+    p.tokens_per_block = tokens_per_block(p, READ, planes, elems);
     for (int i = 0; i < planes; ++i) {
         const uint64_t lanes = (uint64_t)p.plane[i].dim / elems, chunks = lanes * (uint64_t)p.head_k;
         p.plane[i].lanes_magic = (uint32_t)(((1ull << 32) + lanes - 1) / lanes);
