@@ -11,6 +11,11 @@
 // a row are small multiples of one power of two, and so is max - min), and there the bits of a float32 quotient would
 // decide which of the two is stored.  scale and zero are rounded to float32 first, since n has to fit the pair that is
 // stored.
+//
+// What bounds them: a read moves 5 to 6 TB/s, as much as a copy (24 sequences of 0 .. 1300 tokens, 16-bit, 4 heads d 256: 131 MB in
+// 23 to 27 us; 114 000 int4 tokens of 8 heads d 128 with a pair per 64: 615 MB in 119 to 135).  An append spends 12 vector
+// instructions an element on exact quotients and runs at 4.3 TB/s (26 000 tokens of 8 heads d 128, int8 per 64: 168 MB in 39 us).
+// Small calls are the launch and the three trips of the look-up: 3 to 4 us, for one sequence or 64.
 #include "da_kv_cache.h"
 
 namespace da {
@@ -202,12 +207,12 @@ __device__ __forceinline__ float not_finite(uint4 w, float seen) {
 }
 
 // The same for ordinary values at a fourth of the instructions, sixteen integers packed into four words (int4: two).
-// One multiply-add in double precision, x inv + (zero + 1/2 + a constant of 1.5 2^28 or 1.5 2^24), leaves t + 1/2 in the low word as
-// a fixed-point number in units of 2^-24 (int8) or 2^-28 (int4), the integer in its upper bits.  It is off by a unit at most, half
-// from the sum in brackets and half from the result (inv, and the definition's quotient and sum, by less than 2^-40: |zero| < 2^20),
-// and two are added: a fraction of five units and more lies behind the whole number that the definition rounds to, and one that
-// passed the next whole number counts three at most.  The others (of normal values, a lane's sixteen in 200) are settled by the
-// quotient itself.
+// One multiply-add in double precision, x inv + (zero + 1/2 + a constant of 1.5 2^28 or 1.5 2^24), leaves t + 1/2 in the low
+// word as a fixed-point number in units of 2^-24 (int8) or 2^-28 (int4), the integer in its upper bits.  It is off by a unit at
+// most, half from the sum in brackets and half from the result (inv, and the definition's quotient and sum, by less than 2^-40:
+// |zero| < 2^20), and two are added: a fraction of five units and more lies behind the whole number that the definition rounds
+// to, and one that passed the next whole number counts three at most.  The others (of normal values, a lane's sixteen in 200)
+// are settled by the quotient itself.
 template <typename Tag, int FMT, int PAIRS>
 __device__ __forceinline__ void quantise(const uint4 (&raw)[2], const uint16_t* src, float factor, int span, uint32_t (&w)[4],
                                          float2& pair) {
@@ -482,10 +487,10 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const KvCacheParams p
     }
 }
 
-// Tokens per work-group: a thread holds up to kUnroll chunks, fewer while that leaves CUs without a work-group.  Large calls
-// take two turns, for the rows' look-up is three trips to memory one after the other: int8 with a pair per 64, 26 000 tokens of
-// 8 heads d 128, 47.2 -> 39.2 us with half the work-groups; a read looks up less beside more bytes, int4 per 64, 114 000 tokens, 138 ->
-// 132 us, and 29.5 -> 30.0 at a quarter of that.
+// Tokens per work-group: a thread holds up to kUnroll chunks, fewer while that leaves CUs without a work-group.  Large calls take
+// two turns, for the rows' look-up is three trips to memory one after the other: int8 with a pair per 64, 26 000 tokens of 8
+// heads d 128, 47.2 -> 39.2 us with half the work-groups; a read gains less, int4 per 64, 114 000 tokens, 138 -> 132 us, and at
+// 26 000 it loses, 29.5 -> 30.0.
 int tokens_per_block(const KvCacheParams& p, bool read, int planes, int elems) {
     const int chunks = p.head_k * (p.plane[0].dim >> 3);  // (of eight elements: kUnroll of them to a thread)
     int tpb = kThreads * kUnroll / chunks;

@@ -10,13 +10,24 @@
 // Both leave un-normalised partials (o, m, l); the merge kernel adds them up: with M = max m_i,
 //   o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i.
 //
-// A prefix work-group: wave w holds Q rows 32 w .. + 31 in registers as B-operands of v_mfma_f32_32x32x16.  K and V tiles
-// go from global memory straight to LDS, two buffers, the next tile in flight behind the one being used.  Per tile
+// A prefix work-group: wave w holds Q rows 32 w .. + 31 in registers as B-operands of v_mfma_f32_32x32x16.  K and V tiles of
+// 32 tokens go from global memory straight to LDS, three buffers each, two tiles in flight behind the one being used.  Per tile
 //   S^T[tok x 32 rows] = K . Q^T       (A: K rows from LDS, 16 bytes a lane)
 //   P^T = 2^(S^T scale - m)            one row per lane pair (lane, lane + 32): sums and maxima stay in the lane
 //   O^T[col x 32 rows] += V^T . P^T    (A: V through transposed LDS reads; P^T is a B-operand as it lies)
 // The k order of the second product is the score tile's: lane half h holds tokens 4 h .. + 3 and 8 + 4 h .. + 3 of every
-// sixteen.
+// sixteen.  The loop is skewed: the scores of tile u + 1 run beside the exponentials of tile u, and its value products beside
+// the next maximum and the K fragments of tile u + 2.  The running maximum moves only when a score exceeds it by 2^8, so that the
+// accumulators are rarely rescaled (weights up to 2^8 lose nothing: sums are float32, and P's 16 bits are relative).
+// P is rounded to 16 bits for the second product, as everywhere in this library; the denominator sums the rounded values, so
+// that a row's weights still add up to one.
+//
+// What bounds it: the prefix part alone is power-limited matrix work, 256 sequences behind 16384 tokens, 32/8 heads d 128:
+// 80 us, 860 TFLOP/s at 1.75 GHz with two work-groups per CU; with one per CU it is the latency of a tile's chain (0.6 us for
+// 0.25 us of products).  With own tokens (542 MB) the launch takes 141 us, 3.8 TB/s and 490 TFLOP/s together, where one part after
+// the other takes 175.  128 rows a work-group: with 64 the K/V reads from LDS per product double, with 256 the splits, and so the
+// partials, do.  Wide rows (d 256) leave one work-group per CU and its chain: 1056 rows behind 32768 tokens 55 us, 640
+// TFLOP/s; there the partials' way out and back is a third of a short call (8192 tokens: 12 of 36 us).
 #pragma once
 #include "da_gqa_mfma.h"
 #include "da_mla_dev.h"
