@@ -336,7 +336,7 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         auto pack = [&](int j) __attribute__((always_inline)) { pw[j] = EL::pack2(e[2 * j], e[2 * j + 1]); };
         // Exponentials up to kEarly go out beside the score products, the rest beside the first value products; a pair is packed
         // a slot after its second one.
-        constexpr int kPre = 0, kEarly = 12;
+        constexpr int kPre = 0, kEarly = 16;
         auto exps = [](int slot, int slots, int from, int to) { return from + (to - from) * slot / slots; };
         auto packs = [&](int from, int to) __attribute__((always_inline)) {  // pairs of exponentials [from, to)
 #pragma unroll
