@@ -1420,10 +1420,11 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
     pl.groups = (int)((ratio + 15) / 16);
     pl.own_groups = (int)(pl.wave_per_head ? head_k / 4 : head_k) * pl.groups;
     // Splits of the prefix, by the expected time of both parts and of the partials' way out and back.  A prefix work-group takes
-    // 10 us and `step` per 32-token tile, 1.7 times that beside own work-groups (32/8 heads d 128, 16384 tokens: 0.61 and 1.1 us;
-    // d 64 0.48 and 0.75; d 256 0.85 alone) or beside a second one.  Up to d = 128 a CU holds one of each kind, or two; at
-    // d = 256 one.  The row tiles of a (KV head, split) pair are kept on one XCD unless dealing them out over all eight is
-    // faster with the K/V read into every L2 (64/2 heads d 128, 82 sequences behind 5120 tokens: 21 row tiles a pair, 48 -> 38 us).
+    // 6 us and `step` per 32-token tile, 1.7 times that beside own work-groups (32/8 heads d 128, 16384 tokens: 0.61 and 1.1 us;
+    // d 64 0.48 and 0.75; d 256 0.85 alone) or beside a second one; while both run the own ones lose a fifth.  Up to d = 128 a
+    // CU holds one of each kind, or two; at d = 256 one.  The row tiles of a (KV head, split) pair are kept on one XCD unless
+    // dealing them out over all eight is faster with the K/V read into every L2 (64/2 heads d 128, 82 sequences behind 5120
+    // tokens: 21 row tiles a pair, 48 -> 38 us).
     pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
     const double own_us = own_max > 0 ? 4.0 * (double)own_total * (double)head_k * (double)dim / 5.0e6 + 6.0 : 0.0;
     const double kv_us = 4.0 * (double)prefix_len * (double)head_k * (double)dim / 5.0e6;
@@ -1440,7 +1441,7 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
         for (int spread = 0; spread < 2; ++spread) {
             const long long per_xcd =
                 spread ? ((long long)head_k * s * pl.row_tiles + 7) / 8 : ((long long)head_k * s + 7) / 8 * pl.row_tiles;
-            const double start = 10.0 + (spread ? 8.0 * kv_us / 4.0 : kv_us) / 2.0;
+            const double start = 6.0 + (spread ? 8.0 * kv_us / 4.0 : kv_us) / 2.0;
             const double one = (double)((per_xcd + 31) / 32 * tiles), two = (double)((per_xcd + 63) / 64 * tiles);  // steps in a row
             double us;
             bool share_cus = false;
