@@ -36,6 +36,11 @@ struct Place {
 };
 constexpr int64_t kNowhere = -1, kBehind = -2;
 
+// Evenly spaced sequences: their entries of cu_seq, and their lengths.
+struct Marks {
+    int32_t start[kThreads], len[kThreads];
+};
+
 // Row of the pools where token t lies, kNowhere if it lies nowhere: a token's sequence ends at seq_lens[b], and the tokens of
 // the call are its last ones.  Bounds are checked here, for the row is written: a position before the sequence's first
 // token (a padded sequence of no tokens), behind the block table, or a page that the pools do not have.
@@ -47,10 +52,9 @@ __device__ __forceinline__ int64_t pool_row(const KvCacheParams& p, int b, int64
 }
 
 // Looks the work-group's rows up, one thread a token.  The sequence of a token is found among 256 evenly spaced entries of
-// cu_seq, fetched by the threads at once and searched in LDS, and then between two of them: with up to 256 sequences one trip
-// to memory where a search in memory takes eight.
-__device__ __forceinline__ void find_rows(const KvCacheParams& p, const KvPlane& pl, int64_t tok0, Place* places,
-                                          int32_t* marks) {
+// cu_seq, fetched by the threads at once (and the lengths with them) and searched in LDS, and then between two of them: with up
+// to 256 sequences one trip to memory, in front of the block table's, where a search in memory takes eight.
+__device__ __forceinline__ void find_rows(const KvCacheParams& p, const KvPlane& pl, int64_t tok0, Place* places, Marks& marks) {
     const int64_t t = tok0 + threadIdx.x;
     const bool mine = (int)threadIdx.x < p.tokens_per_block && t < p.tokens;
     int64_t row = kBehind;
@@ -58,25 +62,31 @@ __device__ __forceinline__ void find_rows(const KvCacheParams& p, const KvPlane&
         if (mine) row = pool_row(p, (int)t, (int64_t)p.seq_lens[t] - 1);
     } else {
         const int step = (p.batch + kThreads - 1) / kThreads;
-        marks[threadIdx.x] = p.cu_seq[min((int)threadIdx.x * step, p.batch)];
+        marks.start[threadIdx.x] = p.cu_seq[min((int)threadIdx.x * step, p.batch)];
+        marks.len[threadIdx.x] = p.seq_lens[min((int)threadIdx.x * step, p.batch - 1)];
         const int32_t end = p.cu_seq[p.batch];
         __syncthreads();
-        if (mine && t >= marks[0] && t < end) {
+        if (mine && t >= marks.start[0] && t < end) {
             int lo = 0;  // the last mark at or below t
             for (int half = kThreads / 2; half > 0; half >>= 1)
-                if (marks[lo + half] <= t) lo += half;
-            lo *= step;
-            int n = min(step, p.batch - lo);  // cu_seq[lo] <= t < cu_seq[lo + n]
-            while (n > 1) {
-                const int half = n >> 1;
-                if (p.cu_seq[lo + half] <= t) {
-                    lo += half;
-                    n -= half;
-                } else {
-                    n = half;
+                if (marks.start[lo + half] <= t) lo += half;
+            int64_t len = marks.len[lo], next = lo + 1 < kThreads ? marks.start[lo + 1] : end;
+            if (step > 1) {
+                lo *= step;
+                int n = min(step, p.batch - lo);  // cu_seq[lo] <= t < cu_seq[lo + n]
+                while (n > 1) {
+                    const int half = n >> 1;
+                    if (p.cu_seq[lo + half] <= t) {
+                        lo += half;
+                        n -= half;
+                    } else {
+                        n = half;
+                    }
                 }
+                len = p.seq_lens[lo];
+                next = p.cu_seq[lo + 1];
             }
-            row = pool_row(p, lo, (int64_t)p.seq_lens[lo] - (p.cu_seq[lo + 1] - t));
+            row = pool_row(p, lo, len - (next - t));
         }
     }
     if ((int)threadIdx.x < p.tokens_per_block)
@@ -339,7 +349,7 @@ template <typename Tag, int FMT, int PAIRS>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvCacheParams p) {
     constexpr int E = append_chunk<FMT>(), V = E / 8, U = kUnroll / V;  // V: 16-byte loads of a chunk
     __shared__ Place places[kMaxTokens];
-    __shared__ int32_t marks[kThreads];
+    __shared__ Marks marks;
     const KvPlane& pl = p.plane[blockIdx.y];
     const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;
     const int lanes = pl.dim / E, chunks = p.head_k * lanes;
@@ -418,7 +428,7 @@ template <typename Tag, int FMT, int PAIRS>
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(const KvCacheParams p) {
     using EL = Elem<Tag>;
     __shared__ Place places[kMaxTokens];
-    __shared__ int32_t marks[kThreads];
+    __shared__ Marks marks;
     const KvPlane& pl = p.plane[blockIdx.y];
     const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;
     const int lanes = pl.dim >> 3, chunks = p.head_k * lanes;

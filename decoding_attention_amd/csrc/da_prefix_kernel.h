@@ -550,7 +550,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
         for (int n = w.batch; n > 1;) {  // the last b with cu[b] <= r0: 64 probes at once
             const int stride = (n + 63) >> 6;
             const int idx = b + (int)(threadIdx.x & 63) * stride;
-            const int k = __popcll(__ballot(idx < b + n && cu[idx] <= r0)) - 1;
+            const int k = max(__popcll(__ballot(idx < b + n && cu[idx] <= r0)), 1) - 1;
             b += k * stride;
             n = min(stride, n - k * stride);
         }

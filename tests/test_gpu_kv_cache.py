@@ -160,7 +160,7 @@ def test_one_token_per_sequence_and_padded_rows(fmt):
     c.check_read(c.read())
 
 
-@pytest.mark.parametrize("batch", [1, 2, 63, 64, 65, 300])
+@pytest.mark.parametrize("batch", [1, 2, 63, 64, 65, 255, 256, 257, 300])
 def test_many_sequences_with_empty_ones_between(batch):
     g = torch.Generator().manual_seed(batch)
     new = torch.randint(0, 4, (batch,), generator=g)
