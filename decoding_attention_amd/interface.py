@@ -205,7 +205,6 @@ def decoding_attn_shared_prefix_fwd(q: torch.Tensor, k_prefix: torch.Tensor, v_p
     Return:
         o: [batch, head_q, dim_v], same dtype as q.
     """
-    q, k_prefix, v_prefix, k, v = [maybe_contiguous(x) for x in (q, k_prefix, v_prefix, k, v)]
     return _extension().fwd_prefix(q, k_prefix, v_prefix, k, v, out, cu_seq_k, int(max_seq_k), int(dim_v), bool(is_alibi),
                                    None if softmax_scale is None else float(softmax_scale), alibi_slopes)
 
@@ -229,7 +228,6 @@ def decoding_attn_paged_shared_prefix_fwd(q: torch.Tensor, k_pages: torch.Tensor
     Return:
         o: [batch, head_q, dim_v], same dtype as q.
     """
-    q = maybe_contiguous(q)
     return _extension().fwd_paged_prefix(q, k_pages, v_pages, out, prefix_blocks, int(prefix_len), block_table, seq_lens,
                                          int(max_seq_k), int(dim_v), bool(is_alibi),
                                          None if softmax_scale is None else float(softmax_scale), alibi_slopes,
@@ -256,10 +254,6 @@ def kv_cache_append(k: torch.Tensor, v: Optional[torch.Tensor], k_pages: torch.T
             quotients in float64).
     A page that is written must belong to one sequence.
     """
-    if k.stride(-1) != 1:
-        k = k.contiguous()
-    if v is not None and v.stride(-1) != 1:
-        v = v.contiguous()
     _extension().kv_append(k, v, k_pages, v_pages, block_table, seq_lens, cu_seq, k_scale, v_scale)
 
 
