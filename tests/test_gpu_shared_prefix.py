@@ -143,6 +143,23 @@ def test_alibi_and_scale(d, hq, hk, custom):
     check(o, reference(q, kp, vp, ks, vs, True, scale, slopes))
 
 
+@pytest.mark.parametrize("page", [0, 4, 16, 64])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_alibi_over_many_tiles(d, page):
+    """Splits of many tiles and a last one that is cut; flat, steep and falling slopes."""
+    heads, batch = 64, 3
+    prefix = {0: 3003, 4: 3004, 16: 2992, 64: 2944}[page]
+    q, kp, vp, ks, vs = make(batch, heads, heads, d, prefix, [0, 3, 40], torch.float16 if d == 64 else torch.bfloat16, seed=d + page)
+    slopes = torch.linspace(-0.02, 0.8, heads)
+    if page:
+        pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=page)
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, lens, most, d, True, alibi_slopes=slopes.to(DEV))
+    else:
+        k, v, cu, most = packed(ks, vs, heads, d, q.dtype)
+        o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, True, alibi_slopes=slopes.to(DEV))
+    check(o, reference(q, kp, vp, ks, vs, True, None, slopes))
+
+
 @pytest.mark.parametrize("page", [1, 2, 8, 16, 32, 64, 256])
 @pytest.mark.parametrize("d,hq,hk,alibi", [(128, 16, 4, False), (64, 6, 2, True), (96, 8, 8, False), (256, 33, 1, True)])
 def test_pages(d, hq, hk, alibi, page):
