@@ -1409,7 +1409,8 @@ struct PrefixPlan {
     size_t flat_cu_bytes = 0, ws_bytes = 0;
 };
 
-// own_max: most own tokens of a sequence; own_total: all own tokens, 0 = unknown.
+// own_max: most own tokens of a sequence, a bound like any other (the last split takes what lies past it); 0 = no sequence can
+// have any, and no part is planned for them.  own_total: all own tokens, 0 = unknown.
 PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total, size_t batch, size_t head_q, size_t head_k,
                             size_t dim, size_t page_size) {
     PrefixPlan pl;
@@ -1539,7 +1540,9 @@ int run_shared_prefix(const void* q, const void* pk, const void* pv, const int32
     if (!q) return fail(DA_ERR_INVALID_ARGUMENT, "q is null");
     if (!o) return fail(DA_ERR_INVALID_ARGUMENT, "o is null");
     if (!pk || !pv) return fail(DA_ERR_INVALID_ARGUMENT, "the prefix's K or V is null");
-    if (own_max > 0 && (!k || !v)) return fail(DA_ERR_INVALID_ARGUMENT, "k or v is null");
+    if ((own_max > 0 || k || v) && (!k || !v)) return fail(DA_ERR_INVALID_ARGUMENT, "k or v is null");
+    // (rows with a bound of zero: the lengths on the device decide)
+    if (k && own_max == 0) own_max = 1;
     if (!aligned16(q) || !aligned16(pk) || !aligned16(pv) || !aligned16(k) || !aligned16(v) || !aligned16(o))
         return fail(DA_ERR_INVALID_ARGUMENT, "q, o and all K and V must be 16-byte aligned");
     if (batch == 0) return DA_OK;
@@ -1678,9 +1681,12 @@ size_t da_workspace_bytes_shared_prefix(size_t prefix_len, size_t max_seq_k, siz
     if (head_k == 0 || head_q % head_k != 0 || !supported_dims(dim, dim_v) || dim != dim_v || batch == 0) return 0;
     if (prefix_len == 0) return plan_ws_bytes(max_seq_k, batch, head_q, head_k, dim, dim_v, true, total_k, page_size);
     const size_t own = page_size == 0 ? max_seq_k : (max_seq_k > prefix_len ? max_seq_k - prefix_len : 0);
-    return make_prefix_plan(prefix_len, own, page_size == 0 ? total_k : own_tokens(total_k, prefix_len, batch), batch, head_q,
-                            head_k, dim, page_size)
-        .ws_bytes;
+    const size_t total = page_size == 0 ? total_k : own_tokens(total_k, prefix_len, batch);
+    const auto bytes = [&](size_t most) {
+        return make_prefix_plan(prefix_len, most, total, batch, head_q, head_k, dim, page_size).ws_bytes;
+    };
+    // (a bound of zero: the call may come with rows or without)
+    return own > 0 ? bytes(own) : std::max(bytes(0), bytes(1));
 }
 
 }  // extern "C"

@@ -361,6 +361,8 @@ int da_kv_cache_read(const void *k_pages, const void *v_pages, void *k, void *v,
  *           the prefix (a whole number of pages) is read through prefix_blocks (int32, prefix_len / page_size page ids), and
  *           the first prefix_len / page_size entries of the block table's rows are not read.  A sequence shorter than the
  *           prefix (a padded row of the batch, length 0) gets zero output rows.
+ * max_seq_k and total_k plan the work and nothing else: where they are too low, zero included, every token that the lengths on
+ * the device name is attended to all the same.
  * prefix_len == 0 is the call without a prefix.  Workspace from da_workspace_bytes_shared_prefix (page_size 0 = packed).
  */
 int da_decoding_attn_shared_prefix(const void *q, const void *k_prefix, const void *v_prefix, size_t prefix_len,

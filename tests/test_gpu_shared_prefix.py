@@ -488,3 +488,49 @@ def test_pages_past_32_bit_offsets(page):
     table = torch.where(table >= 0, where[table.clamp(min=0).long()], -1).to(torch.int32)
     o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), *big, where[ids.long()].to(torch.int32), prefix, table, lens, most, d, False)
     check(o, reference(q, kp, vp, ks, vs, False))
+
+
+@pytest.mark.parametrize("lengths", [OWN, LONG_OWN], ids=["short", "long"])
+@pytest.mark.parametrize("page", [0, 1, 16, 64])
+def test_bounds_below_the_lengths_drop_no_token(page, lengths):
+    """A bound on the lengths that is too low, down to the prefix's own length (no own token at all) and to zero: the tokens that
+    the device's lengths name are attended to all the same."""
+    prefix, hq, hk, d = 192, 16, 4, 128
+    q, kp, vp, ks, vs = make(len(lengths), hq, hk, d, prefix, lengths, torch.bfloat16, seed=30 + page)
+    rows = [0, 1, 2, 4, 6, 7]
+    ref = some(q, kp, vp, ks, vs, False, rows)
+    if page:
+        pk, pv, ids, table, lens, _ = paged(kp, vp, ks, vs, page, seed=page)
+        for bound in (0, 1, prefix, prefix + 1, prefix + 40):
+            for total in (0, int(lens.sum())):
+                o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, lens, bound, d, False, total_k=total)
+                check(o[rows], ref)
+    else:
+        k, v, cu, _ = packed(ks, vs, hk, d, torch.bfloat16)
+        for bound in (0, 1, 40):
+            o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, bound, d, False)
+            check(o[rows], ref)
+
+
+def test_entry_point_with_a_bound_of_zero():
+    """The C call with rows and max_seq_k 0 attends to them; with max_seq_k 0 and no rows the prefix is all there is.  The
+    workspace that the query names for a bound of zero covers both."""
+    from decoding_attention_amd import _lib
+    lib = _lib.load()
+    for prefix in (300, 5000):
+        q, kp, vp, ks, vs = make(8, 16, 4, 128, prefix, OWN, torch.float16, seed=31)
+        k, v, cu, _ = packed(ks, vs, 4, 128, torch.float16)
+        dq, dkp, dvp = q.to(DEV), kp.to(DEV), vp.to(DEV)
+        need = lib.da_workspace_bytes_shared_prefix(prefix, 0, 8, 16, 4, 128, 128, 0, 0)
+        none = [t[:0] for t in ks]
+        for rows in (True, False):
+            ws = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+            o = torch.full((8, 16, 128), float("nan"), dtype=torch.float16, device=DEV)
+            at = cu if rows else torch.zeros_like(cu)
+            rc = lib.da_decoding_attn_shared_prefix(
+                dq.data_ptr(), dkp.data_ptr(), dvp.data_ptr(), prefix, k.data_ptr() if rows else None,
+                v.data_ptr() if rows else None, o.data_ptr(), at.data_ptr(), 0, 8, 16, 4, 128, 128, 0, 0, 0.0, None, 0,
+                ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream)
+            assert rc == 0, _lib.last_error()
+            torch.cuda.synchronize()
+            check(o, reference(q, kp, vp, ks if rows else none, vs if rows else none, False))

@@ -129,3 +129,16 @@ def test_python_face_rejects_cpu_tensors_and_types():
         da.decoding_attn_shared_prefix_fwd(k, k, k, k, k, cu, 1, 64, False)
     with pytest.raises(RuntimeError, match="must be on the GPU"):
         da.decoding_attn_paged_shared_prefix_fwd(k, pool, pool, table[0], 16, table, lens, 16, 64, False)
+
+
+def test_prefix_bound_of_zero():
+    """Rows come as K and V or not at all, and the workspace for a bound of zero is enough for either."""
+    lib = _lib.load()
+    inv = _lib.DA_ERR_INVALID_ARGUMENT
+    assert _prefix(lib, most=0, k=None) == inv and _prefix(lib, most=0, v=None) == inv
+    for prefix in (1, 300, 5000, 16384):
+        for batch in (1, 8, 200):
+            zero = lib.da_workspace_bytes_shared_prefix(prefix, 0, batch, 32, 8, 128, 128, 0, 0)
+            assert zero >= 2 * batch * 32 * 130 * 4
+            one = lib.da_workspace_bytes_shared_prefix(prefix, 1, batch, 32, 8, 128, 128, 0, 0)
+            assert zero >= one
