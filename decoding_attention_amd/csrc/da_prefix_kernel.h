@@ -120,24 +120,27 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
     const int last = c1 - 1, nu = (c1 - c0 + kTok - 1) / kTok;
     // Tile number u starts at token at0 + u * ahead.  With ALiBi the last tokens come first: their bias is the highest (of
     // positive slopes), and in the other order a steep head would raise its maximum, and rescale, in every tile (33 sequences
-    // behind 8192 tokens, 32/1 heads d 256: 88.8 -> 39.4 us; 256 behind 16384, 32/8 heads d 128: 172 -> 155).
-    const int tile_last = c0 + (nu - 1) * kTok;
-    const int at0 = w.is_alibi ? tile_last : c0, ahead = w.is_alibi ? -kTok : kTok;
+    // behind 8192 tokens, 32/1 heads d 256: 88.8 -> 39.4 us; 256 behind 16384, 32/8 heads d 128: 172 -> 155).  They do as well where
+    // the split's last tile is cut, so that a cut tile is always the first one and the loop has none to look after.
+    const int tile_last = c0 + (nu - 1) * kTok, cut = c1 - tile_last;  // (cut: tokens of the last tile)
+    const bool back = w.is_alibi || cut < kTok;
+    const int at0 = back ? tile_last : c0, ahead = back ? -kTok : kTok;
 
     // Tile loads: a wave fills rows 8 w .. 8 w + 7 of every tile, RPL rows an instruction, 16 bytes a lane, from the address of
     // its first row (one page look-up: its rows lie in one page of 8 tokens and more) and per-lane offsets.  Tokens past the
-    // split's end repeat its last one and are masked.
+    // split's end repeat its last one; their scores are masked, and their V rows cleared (an infinite value of the last token
+    // would be no number under a weight of zero).
     const int lrow = lane / SLOTS, slot = lane % SLOTS;
     const uint32_t row_bytes = (uint32_t)w.k_row * 2;
-    const int first_last = min(tile_last + wave * 8, last);
-    uint32_t off[LOADS], off_end[LOADS];  // of any tile, and of the last one
+    const int first_0 = min(at0 + wave * 8, last);
+    uint32_t off[LOADS], off_0[LOADS];  // of any tile, and of the first one
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
         const int r = wave * 8 + i * RPL + lrow;
         const int c = slot ^ swizzle<D>(r);
         const uint32_t col = (uint32_t)(c < CPR ? c : c - 8) * 16;  // (an empty chunk: any other one of the row)
         off[i] = (uint32_t)(i * RPL + lrow) * row_bytes + col;
-        off_end[i] = (uint32_t)(min(tile_last + r, last) - first_last) * row_bytes + col;
+        off_0[i] = (uint32_t)(min(at0 + r, last) - first_0) * row_bytes + col;
     }
     const uint8_t* const kbase = reinterpret_cast<const uint8_t*>(p.k) + (size_t)hk * D * 2;
     const uint8_t* const vbase = reinterpret_cast<const uint8_t*>(p.v) + (size_t)hk * D * 2;
@@ -154,16 +157,15 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) dma16(at, o[i], lds0 + to + i * 1024);
     };
-    // any tile, that of the last tokens and those past the end (which are not fetched) included
-    auto load = [&](const uint8_t* base, int64_t page_stride, int u, uint32_t to) __attribute__((always_inline)) {
+    // any tile (those past the last one are not fetched); only the first may be cut
+    auto load = [&](const uint8_t* base, int64_t page_stride, int u, uint32_t to, auto first_c) __attribute__((always_inline)) {
         if (u >= nu) return;
         const int tok0 = at0 + u * ahead;
         if (PGM != 2 || page_mask >= 7) {
-            const uint8_t* const at = base + row_at(min(tok0 + wave * 8, last), page_stride);
-            if (tok0 == tile_last)
-                dma_rows(at, off_end, to);
+            if constexpr (decltype(first_c)::value)
+                dma_rows(base + row_at(first_0, page_stride), off_0, to);
             else
-                dma_rows(at, off, to);
+                dma_rows(base + row_at(tok0 + wave * 8, page_stride), off, to);
         } else {  // smaller pages: those of the wave's eight rows, each lane picking its own
             int32_t page[8];
 #pragma unroll
@@ -180,15 +182,15 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             }
         }
     };
-    auto load_k = [&](int u, int buf) __attribute__((always_inline)) { load(kbase, w.k_page, u, buf * TILE); };
-    auto load_v = [&](int u, int buf) __attribute__((always_inline)) { load(vbase, w.v_page, u, (3 + buf) * TILE); };
+    auto load_k = [&](int u, int buf) __attribute__((always_inline)) { load(kbase, w.k_page, u, buf * TILE, std::false_type{}); };
+    auto load_v = [&](int u, int buf) __attribute__((always_inline)) { load(vbase, w.v_page, u, (3 + buf) * TILE, std::false_type{}); };
     // (packed rows: this wave's addresses in the tiles fetched last)
     const int64_t ahead_bytes = (int64_t)ahead * row_bytes;
     const uint8_t* k_next = kbase + (int64_t)(at0 + 3 * ahead + wave * 8) * row_bytes;
     const uint8_t* v_next = vbase + (int64_t)(at0 + ahead + wave * 8) * row_bytes;
-    load_k(0, 0);
+    load(kbase, w.k_page, 0, 0, std::true_type{});
     load_k(1, 1);
-    load_v(0, 0);
+    load(vbase, w.v_page, 0, 3 * TILE, std::true_type{});
     load_k(2, 2);
     load_v(1, 1);
 
@@ -245,13 +247,13 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
         return mx;
     };
-    // ALiBi and the mask of tokens past the end, the running maximum, and (rarely) the rescaling it asks for; mx: max_of(s)
-    const int plain_tiles = w.is_alibi ? 0 : (c1 - c0) / kTok;  // tiles before the first that needs either
+    // ALiBi and (the first tile) the mask of tokens past the end, the running maximum, and (rarely) the rescaling it asks for;
+    // mx: max_of(s)
     auto settle_max = [&](int u, float mx, auto first_c) __attribute__((always_inline)) {
-        if (u >= plain_tiles) {
-            const int tok0 = at0 + u * ahead + 4 * h;
+        constexpr bool first = decltype(first_c)::value;
+        if (first ? back : (bool)w.is_alibi) {
             if (w.is_alibi) {
-                const float at = slope * (float)(tok0 - end);
+                const float at = slope * (float)(at0 + u * ahead + 4 * h - end);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const int j = (i >> 2) * 8 + (i & 3);
@@ -259,15 +261,15 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
                 }
                 mul = 1.0f;
             }
-            if (at0 + u * ahead + kTok > c1) {
+            if constexpr (first) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (tok0 + (i >> 2) * 8 + (i & 3) >= c1) s[i] = -INFINITY;
+                    if (4 * h + (i >> 2) * 8 + (i & 3) >= cut) s[i] = -INFINITY;
             }
             mx = max_of(s);
         }
         mx = max_xor32(mx) * mul;
-        if constexpr (decltype(first_c)::value) {  // (nothing to rescale yet)
+        if constexpr (first) {  // (nothing to rescale yet)
             m = mx > kNegBig ? mx : kNegBig;
             return;
         }
@@ -413,6 +415,16 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) read_k(ks, 0);
     s = scores(kf);
+    if (cut < kTok) {  // this wave's V rows past the end, once they have landed (the barrier of the first step follows)
+        if (nu > 2)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * LOADS) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            if (wave * 8 + i * RPL + lrow >= cut)
+                *reinterpret_cast<uint4*>(smem + 3 * TILE + (wave * LOADS + i) * 1024 + lane * 16) = make_uint4(0u, 0u, 0u, 0u);
+    }
     if (nu > 2)
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(3 * LOADS) : "memory");
     else

@@ -534,3 +534,50 @@ def test_entry_point_with_a_bound_of_zero():
             assert rc == 0, _lib.last_error()
             torch.cuda.synchronize()
             check(o, reference(q, kp, vp, ks if rows else none, vs if rows else none, False))
+
+
+def check_infinite(got, ref, at):
+    """As check(), with entries (sequence or slice, heads, column, +-inf) that have to be that infinity."""
+    got = got.cpu().clone()
+    for b, heads, col, value in at:
+        assert (got[b, heads, col] == value).all(), got[b, heads, col]
+        got[b, heads, col] = 0
+        ref[0][b, heads, col] = 0
+    check(got, ref)
+
+
+@pytest.mark.parametrize("alibi", [False, True])
+@pytest.mark.parametrize("prefix,page", [(1, 0), (31, 0), (33, 0), (77, 0), (100, 0), (1001, 0), (5, 1), (100, 4), (1004, 4), (48, 16)])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_an_infinite_value_in_the_prefixs_last_token(d, prefix, page, alibi):
+    """Every sequence gives it weight, so that it is infinite in its column of the KV head's rows and nowhere else: what fills up
+    the last tile of a prefix that is no multiple of 32 tokens has weight zero, and zero times infinity is no number."""
+    hq, hk, dtype = 12, 3, torch.bfloat16 if prefix % 2 else torch.float16
+    q, kp, vp, ks, vs = make(5, hq, hk, d, prefix, [0, 3, 40, 1, 0], dtype, seed=prefix + d)
+    vp[-1, 1, 3] = vp[-1, 1, d - 1] = 0.0
+    slopes = torch.full((hq,), 0.02) if alibi else None
+    ref = reference(q, kp, vp, ks, vs, alibi, None, slopes)
+    vp[-1, 1, 3], vp[-1, 1, d - 1] = float("inf"), -float("inf")
+    dslopes = slopes.to(DEV) if alibi else None
+    if page:
+        pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=page)
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, lens, most, d, alibi, alibi_slopes=dslopes)
+    else:
+        k, v, cu, most = packed(ks, vs, hk, d, dtype)
+        o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, alibi, alibi_slopes=dslopes)
+    check_infinite(o, ref, [(slice(None), slice(4, 8), 3, float("inf")), (slice(None), slice(4, 8), d - 1, -float("inf"))])
+
+
+@pytest.mark.parametrize("prefix", [1984, 2003])
+@pytest.mark.parametrize("falling", [False, True])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_a_maximum_that_moves_in_splits_of_many_tiles(d, falling, prefix):
+    """Keys in the order of their scores, up or down, in splits whose last tile is whole or cut: from either end of a split the
+    running maximum is raised again and again, and the values far from it still count for nothing."""
+    heads = 64
+    q, kp, vp, ks, vs = make(3, heads, heads, d, prefix, [0, 3, 40], torch.bfloat16, seed=5 + d, sharp=0.1)
+    ramp = torch.linspace(-60, 60, prefix)
+    q[:, :, 0], kp[:, :, 0] = 8.0, (ramp.flip(0) if falling else ramp).bfloat16()[:, None]
+    k, v, cu, most = packed(ks, vs, heads, d, torch.bfloat16)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
+    check(o, reference(q, kp, vp, ks, vs, False))
