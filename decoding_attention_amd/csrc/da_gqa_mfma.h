@@ -127,7 +127,10 @@ constexpr size_t gqa_lds_bytes(int nt, int tok_pairs = 0) {
 // PGM: how paged K/V is addressed.  0: one page lookup per tile (pages hold a multiple of 32 tokens; also the packed
 // layout); 1: 16-token pages, a tile is fetched as two runs of 16 tokens, each from one page; 2: smaller pages, every
 // lane looks up the page of the row it loads.
-template <typename Tag, int D, int DV, int NT, bool PREFETCH, bool WH, int KV8, int PGM>
+// CLEAR: V rows past the end become zeros in the tile, so that an infinite value of the last token, which they repeat, stays
+// infinite (zero times infinity is no number).  Behind a shared prefix only, where the registers are the prefix's; here they
+// would cost the kernels at d = 256 up to 60 bytes more of scratch a lane.
+template <typename Tag, int D, int DV, int NT, bool PREFETCH, bool WH, int KV8, int PGM, bool CLEAR = false>
 __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const smem, const int by, const int b,
                                             const int start, const int len, const int c0, const int c1,
                                             const size_t part0, const int part_stride, const bool direct) {
@@ -178,6 +181,7 @@ __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const
     static_assert(!VK || (DV < D && DV % 64 == 0), "value columns inside the key rows");
     static_assert(D % 32 == 0 && DV % 16 == 0 && (kGqaTile * CPR) % 64 == 0, "shape");
     static_assert(!KV8 || (D % 64 == 0 && (kGqaTile * CPRL) % 64 == 0), "8-bit K/V: two k-steps per 16-byte load");
+    static_assert(!CLEAR || (KV8 == 0 && !VK), "16-bit V of its own");
     static_assert(!TOK || (!VK && (FMT == kKvInt8 || FMT == kKvInt4)), "per-token factors: integer K/V, V of its own");
 
     const int lane = threadIdx.x & 63;
@@ -418,6 +422,15 @@ __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const
                     convert8(make_uint2(tr.v[i].z, tr.v[i].w));
             } else {
                 *reinterpret_cast<uint4*>(vt + row * VP + ch * 16) = tr.v[i];
+            }
+        }
+        if constexpr (CLEAR) {
+            if (tok0 + kGqaTile > c1) {
+                int at = (int)threadIdx.x;  // (the lane's number anew: no register of the loop is kept for this)
+                asm volatile("" : "+v"(at));
+#pragma unroll 1
+                for (at = (c1 - tok0) * VP + (at & 63) * 16; at < kGqaTile * VP; at += 64 * 16)
+                    *reinterpret_cast<uint4*>(vt + at) = make_uint4(0u, 0u, 0u, 0u);
             }
         }
         // The K registers of this tile, the only loads still in flight, are needed right after: wait for them here,

@@ -598,8 +598,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
             c1 = split == w.nsplit - 1 ? len : min(len, c0 + w.chunk);
             part0 = (size_t)b * w.head_q * w.nsplit + split;
         }
-        gqa_segment<Tag, D, D, 1, true, WH, 0, PGM>(p.own, smem, by, b, start, len, c0, c1, part0, w.flat_wgs > 0 ? 1 : w.nsplit,
-                                                    false);
+        gqa_segment<Tag, D, D, 1, true, WH, 0, PGM, true>(p.own, smem, by, b, start, len, c0, c1, part0,
+                                                          w.flat_wgs > 0 ? 1 : w.nsplit, false);
         if (w.flat_wgs == 0) break;
         if (!WH) __syncthreads();  // the merge area of this segment is the V tile area of the next
     }

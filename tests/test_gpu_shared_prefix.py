@@ -581,3 +581,27 @@ def test_a_maximum_that_moves_in_splits_of_many_tiles(d, falling, prefix):
     k, v, cu, most = packed(ks, vs, heads, d, torch.bfloat16)
     o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
     check(o, reference(q, kp, vp, ks, vs, False))
+
+
+@pytest.mark.parametrize("lengths", [[0, 3, 40, 32, 1, 133, 16, 47], LONG_OWN], ids=["short", "long"])
+@pytest.mark.parametrize("page", [0, 1, 16, 64])
+@pytest.mark.parametrize("d,hq,hk", [(64, 4, 4), (96, 12, 3), (128, 16, 4), (256, 33, 1)])
+def test_an_infinite_value_in_a_sequences_last_token(d, hq, hk, page, lengths):
+    """The same among the own tokens: the sequence's own column, and no other sequence's."""
+    prefix, dtype = 64, torch.bfloat16
+    q, kp, vp, ks, vs = make(len(lengths), hq, hk, d, prefix, lengths, dtype, seed=page + d)
+    rows = [1, 2, 3, 4, 5, 6]
+    hit = [b for b in rows if lengths[b] > 0]
+    for b in hit:
+        vs[b][-1, hk - 1, 5] = 0.0
+    ref = some(q, kp, vp, ks, vs, False, rows)
+    for b in hit:
+        vs[b][-1, hk - 1, 5] = float("inf")
+    if page:
+        pk, pv, ids, table, lens, most = paged(kp, vp, ks, vs, page, seed=page)
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk, pv, ids, prefix, table, lens, most, d, False, total_k=int(lens.sum()))
+    else:
+        k, v, cu, most = packed(ks, vs, hk, d, dtype)
+        o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
+    heads = slice((hk - 1) * (hq // hk), hq)
+    check_infinite(o[rows], ref, [(rows.index(b), heads, 5, float("inf")) for b in hit])
