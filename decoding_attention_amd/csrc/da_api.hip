@@ -1404,7 +1404,7 @@ struct PrefixPlan {
     int groups = 0, own_splits = 0, own_chunk = 1, own_groups = 0;
     int flat_wgs = 0, flat_step = 1, flat_min = 1, flat_unit = 1;  // balanced own part (see Plan)
     bool scan = false, spread = false;
-    long long own_wgs = 0;
+    long long own_wgs = 0, merge_wgs = 0;
     size_t prefix_parts = 0, own_parts = 0;  // partial rows of either part
     size_t flat_cu_bytes = 0, ws_bytes = 0;
 };
@@ -1506,6 +1506,8 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
             (pl.flat_wgs ? (long long)pl.flat_wgs : (long long)batch * pl.own_splits) * (pl.own_groups / pl.groups);
         pl.own_wgs = pl.groups > 1 ? (segs + 7) / 8 * 8 * pl.groups : segs;
     }
+    const int merge_rows = da::prefix_merge_rows((int)dim, da::prefix_merge_shares(pl.splits, pl.own_splits));
+    pl.merge_wgs = ((long long)(batch * head_q) + merge_rows - 1) / merge_rows;
     pl.prefix_parts = (size_t)pl.splits * batch * head_q;
     pl.ws_bytes = (pl.prefix_parts + pl.own_parts) * (dim + 2) * sizeof(float) + pl.flat_cu_bytes;
     return pl;
@@ -1517,6 +1519,13 @@ size_t own_tokens(size_t total_k, size_t prefix_len, size_t batch) {
     return total_k == 0 ? 0 : (total_k > prefix_len * batch ? total_k - prefix_len * batch : total_k % prefix_len);
 }
 
+// (the kernels count query rows and positions in 32 bits)
+bool prefix_in_range(size_t prefix_len, size_t max_seq_k, size_t batch, size_t head_q) {
+    return prefix_len <= (size_t)INT32_MAX / 2 && max_seq_k <= (size_t)INT32_MAX / 2 && head_q <= 65535 && batch <= (1u << 24) &&
+           batch * head_q <= ((size_t)1 << 28) && ((max_seq_k + 1023) / 1024) * batch * head_q <= ((size_t)1 << 28);
+}
+bool launchable(const PrefixPlan& pl) { return pl.prefix_wgs + pl.own_wgs <= da::kMaxWgs && pl.merge_wgs <= da::kMaxWgs; }
+
 int check_prefix_shape(size_t prefix_len, size_t max_seq_k, size_t batch, size_t head_q, size_t head_k, size_t dim,
                        size_t dim_v) {
     if (head_k == 0 || head_q == 0 || head_q % head_k != 0)
@@ -1524,9 +1533,7 @@ int check_prefix_shape(size_t prefix_len, size_t max_seq_k, size_t batch, size_t
     if (!supported_dims(dim, dim_v) || dim != dim_v)
         return fail(DA_ERR_UNSUPPORTED, "shared prefix: unsupported head dims (dim %zu, dim_v %zu): supported are (64,64) (96,96) "
                     "(128,128) (256,256)", dim, dim_v);
-    // (the kernels count query rows, positions and work-groups in 32 bits)
-    if (prefix_len > (size_t)INT32_MAX / 2 || max_seq_k > (size_t)INT32_MAX / 2 || head_q > 65535 || batch > (1u << 24) ||
-        batch * head_q > ((size_t)1 << 28) || ((max_seq_k + 1023) / 1024) * batch * head_q > ((size_t)1 << 28))
+    if (!prefix_in_range(prefix_len, max_seq_k, batch, head_q))
         return fail(DA_ERR_INVALID_ARGUMENT, "shape out of range (prefix_len %zu, max_seq_k %zu, batch %zu, head_q %zu)",
                     prefix_len, max_seq_k, batch, head_q);
     return DA_OK;
@@ -1547,8 +1554,9 @@ int run_shared_prefix(const void* q, const void* pk, const void* pv, const int32
         return fail(DA_ERR_INVALID_ARGUMENT, "q, o and all K and V must be 16-byte aligned");
     if (batch == 0) return DA_OK;
     const PrefixPlan pl = make_prefix_plan(prefix_len, own_max, own_total, batch, head_q, head_k, dim, pg.table ? pg.page_size : 0);
-    if (pl.prefix_wgs + pl.own_wgs > (long long)INT32_MAX / 2)
-        return fail(DA_ERR_INVALID_ARGUMENT, "shape out of range (%lld work-groups)", pl.prefix_wgs + pl.own_wgs);
+    if (!launchable(pl))
+        return fail(DA_ERR_INVALID_ARGUMENT, "shape out of range (%lld work-groups, %lld in the merge, %lld a launch)",
+                    pl.prefix_wgs + pl.own_wgs, pl.merge_wgs, da::kMaxWgs);
     hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
     void* ws = workspace;
     if (ws) {
@@ -1682,8 +1690,10 @@ size_t da_workspace_bytes_shared_prefix(size_t prefix_len, size_t max_seq_k, siz
     if (prefix_len == 0) return plan_ws_bytes(max_seq_k, batch, head_q, head_k, dim, dim_v, true, total_k, page_size);
     const size_t own = page_size == 0 ? max_seq_k : (max_seq_k > prefix_len ? max_seq_k - prefix_len : 0);
     const size_t total = page_size == 0 ? total_k : own_tokens(total_k, prefix_len, batch);
+    if (!prefix_in_range(prefix_len, max_seq_k, batch, head_q)) return 0;
     const auto bytes = [&](size_t most) {
-        return make_prefix_plan(prefix_len, most, total, batch, head_q, head_k, dim, page_size).ws_bytes;
+        const PrefixPlan pl = make_prefix_plan(prefix_len, most, total, batch, head_q, head_k, dim, page_size);
+        return launchable(pl) ? pl.ws_bytes : 0;
     };
     // (a bound of zero: the call may come with rows or without)
     return own > 0 ? bytes(own) : std::max(bytes(0), bytes(1));

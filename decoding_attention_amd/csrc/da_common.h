@@ -10,6 +10,7 @@
 namespace da {
 
 constexpr int kWave = 64;          // CDNA4 wavefront width
+constexpr long long kMaxWgs = (1ll << 24) - 1;  // most work-groups of 256 threads in a launch: a grid has fewer than 2^32 threads
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1.0e30f;  // finite stand-in for -inf as the initial running maximum
 

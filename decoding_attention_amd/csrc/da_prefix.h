@@ -8,6 +8,11 @@ namespace da {
 constexpr int kPrefixRows = 128;  // query rows of a prefix work-group: 32 for each of its four waves
 constexpr int kScanBatch = 1024;  // most sequences whose lengths a work-group adds up in LDS
 
+// The merge: threads that share a row's partials (four columns of it each), and rows of a work-group.  (Four from six partials;
+// 4 splits and one own partial of 8192 rows are faster in one.)
+constexpr int prefix_merge_shares(int splits, int own_splits) { return splits + own_splits > 5 ? 4 : 1; }
+constexpr int prefix_merge_rows(int dim, int shares) { return (dim == 96 ? 8 : 1024 / dim) / shares; }
+
 struct PrefixParams {
     SweepParams own;              // the sequences' own tokens; q, o, slopes, scale and head counts serve the prefix too
     const void* k;                // prefix rows [prefix_len, head_k, dim], or the page pools

@@ -14,7 +14,7 @@ namespace {
 template <typename Tag, int D, int G>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(const PrefixParams p) {
     using EL = Elem<Tag>;
-    constexpr int C4 = D / 4, R = (D == 96 ? 8 : 256 / C4) / G;  // R: rows of a work-group
+    constexpr int C4 = D / 4, R = prefix_merge_rows(D, G);
     static_assert(R >= 1 && R * G * C4 <= 256, "shape");
     __shared__ f32x4 nums[G][R][C4];
     __shared__ float2 mls[G][R];
@@ -110,7 +110,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(const PrefixParams p)
 
 template <typename Tag, int D, int G>
 hipError_t launch_one(const PrefixParams& p, hipStream_t stream) {
-    constexpr int R = (D == 96 ? 8 : 256 / (D / 4)) / G;
+    constexpr int R = prefix_merge_rows(D, G);
     const unsigned rows = (unsigned)(p.own.batch * p.own.head_q);
     hipLaunchKernelGGL((prefix_merge_kernel<Tag, D, G>), dim3((rows + R - 1) / R), dim3(256), 0, stream, p);
     return hipGetLastError();
@@ -118,8 +118,7 @@ hipError_t launch_one(const PrefixParams& p, hipStream_t stream) {
 
 template <int D>
 hipError_t launch_dim(const PrefixParams& p, bool is_bf16, hipStream_t stream) {
-    // (four shares from six partials; 4 splits and one own partial of 8192 rows are faster in one)
-    const bool shares = p.splits + (p.own.flat_wgs > 0 ? 1 : p.own.nsplit) > 5;
+    const bool shares = prefix_merge_shares(p.splits, p.own.nsplit) > 1;
     if (is_bf16) return shares ? launch_one<bf16_tag, D, 4>(p, stream) : launch_one<bf16_tag, D, 1>(p, stream);
     return shares ? launch_one<f16_tag, D, 4>(p, stream) : launch_one<f16_tag, D, 1>(p, stream);
 }

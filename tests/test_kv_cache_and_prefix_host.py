@@ -142,3 +142,25 @@ def test_prefix_bound_of_zero():
             assert zero >= 2 * batch * 32 * 130 * 4
             one = lib.da_workspace_bytes_shared_prefix(prefix, 1, batch, 32, 8, 128, 128, 0, 0)
             assert zero >= one
+
+
+def test_prefix_calls_refuse_more_work_groups_than_a_launch_has():
+    """A grid holds fewer than 2^32 threads, 2^24 - 1 work-groups of 256: a shape beyond that in the sweep or in the merge is
+    refused before anything is launched, and the query has no size for it.  (In range: the workspace is what is missing.)"""
+    lib = _lib.load()
+    inv, small = _lib.DA_ERR_INVALID_ARGUMENT, _lib.DA_ERR_WORKSPACE
+    few = dict(ws=16, nb=64)
+    # the merge: sixteen rows a work-group at d 64, eight at 128, four at 256, a quarter of them from six partials
+    for d, most, rc in [(64, 1 << 23, small), (128, 1 << 23, small), (256, 1 << 23, small), (256, 1 << 27, inv)]:
+        for own in (0, 8):
+            assert _prefix(lib, batch=most // 32, hq=32, hk=32, d=d, dv=d, most=own, **few) == rc
+            assert _paged_prefix(lib, batch=most // 32, hq=32, hk=32, d=d, dv=d, most=64 + own, **few) == rc
+    # the sweep: a work-group for every sequence (1024 own tokens of it, KV head)
+    assert _prefix(lib, batch=1 << 24, hq=1, hk=1, d=64, dv=64, most=64, **few) == inv
+    assert _prefix(lib, batch=1 << 22, hq=1, hk=1, d=64, dv=64, most=8, **few) == small
+    assert _prefix(lib, batch=1 << 15, hq=1, hk=1, d=64, dv=64, most=1 << 20, **few) == inv
+    size = lib.da_workspace_bytes_shared_prefix
+    assert size(64, 8, 1 << 22, 32, 32, 256, 256, 0, 0) == 0 and size(64, 64, 1 << 24, 1, 1, 64, 64, 0, 0) == 0
+    assert size(BIG, 8, 2, 8, 4, 128, 128, 0, 0) == 0 and size(64, BIG, 2, 8, 4, 128, 128, 0, 16) == 0
+    assert size(64, 8, BIG, 8, 4, 128, 128, 0, 0) == 0 and size(64, 8, 2, 1 << 17, 1, 128, 128, 0, 0) == 0
+    assert size(64, 8, 1 << 22, 1, 1, 64, 64, 0, 0) > 0
