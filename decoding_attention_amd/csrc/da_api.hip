@@ -1357,6 +1357,10 @@ int run_kv_cache(bool read, const void* k, const void* v, void* k_out, void* v_o
     while (((size_t)1 << p.page_shift) < page_size) ++p.page_shift;
     p.max_blocks = (int)max_blocks_per_seq;
     p.num_pages = (int)num_pages;
+    const int per_wg = da::kv_cache_tokens_per_block(p, read, kv_format, has_v ? 2 : 1);
+    const long long wgs = ((long long)tokens + per_wg - 1) / per_wg;
+    if (wgs > da::kMaxWgs)
+        return fail(DA_ERR_INVALID_ARGUMENT, "tokens (%zu) out of range: %lld work-groups, %lld a launch", tokens, wgs, da::kMaxWgs);
     hipStream_t stream = reinterpret_cast<hipStream_t>(hip_stream);
     const hipError_t e = (read ? da::launch_kv_read : da::launch_kv_append)(p, is_bf16 != 0, kv_format, scale_form,
                                                                              has_v ? 2 : 1, stream);

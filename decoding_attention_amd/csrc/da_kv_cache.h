@@ -29,6 +29,9 @@ struct KvCacheParams {
     int tokens_per_block;
 };
 
+// Tokens of a work-group of 256 threads, from p's tokens, heads and widths.
+int kv_cache_tokens_per_block(const KvCacheParams& p, bool read, int fmt, int planes);
+
 // pairs: 0 = a factor per KV head, 1 = a (scale, zero) pair per row, 2 = a pair per 64 elements; fmt: 0, kKvFp8, kKvInt8,
 // kKvInt4.  planes: 1 (K alone) or 2.
 hipError_t launch_kv_append(const KvCacheParams& p, bool is_bf16, int fmt, int pairs, int planes, hipStream_t stream);

@@ -161,12 +161,9 @@ __device__ __forceinline__ int64_t pair_at(const KvCacheParams& p, const KvPlane
 __device__ __forceinline__ float min_nan(float a, float b) { return (b < a || b != b) ? b : a; }
 __device__ __forceinline__ float max_nan(float a, float b) { return (b > a || b != b) ? b : a; }
 
-// Elements a lane takes at once: a row's factors cost a division in double precision per lane, which sixteen elements share;
-// a copy takes eight.
-template <int FMT>
-constexpr int append_chunk() {
-    return FMT == 0 ? 8 : 16;
-}
+// Elements a lane takes at once.  Append: a row's factors cost a division in double precision per lane, which sixteen elements
+// share; a copy takes eight.
+constexpr int row_chunk(bool read, int fmt) { return read || fmt == 0 ? 8 : 16; }
 
 // The definition as it stands, for what the ways below leave out: values that are not finite, factors outside any sense, and
 // quotients that lie within rounding of half a step.  `span` lanes hold a row or run; `src` are the lane's sixteen values once
@@ -347,7 +344,7 @@ __device__ __forceinline__ void quantise_fp8(const uint4 (&raw)[2], const uint16
 
 template <typename Tag, int FMT, int PAIRS>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvCacheParams p) {
-    constexpr int E = append_chunk<FMT>(), V = E / 8, U = kUnroll / V;  // V: 16-byte loads of a chunk
+    constexpr int E = row_chunk(false, FMT), V = E / 8, U = kUnroll / V;  // V: 16-byte loads of a chunk
     __shared__ Place places[kMaxTokens];
     __shared__ Marks marks;
     const KvPlane& pl = p.plane[blockIdx.y];
@@ -501,7 +498,10 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(const KvCacheParams p
 // two turns, for the rows' look-up is three trips to memory one after the other: int8 with a pair per 64, 26 000 tokens of 8
 // heads d 128, 47.2 -> 39.2 us with half the work-groups; a read gains less, int4 per 64, 114 000 tokens, 138 -> 132 us, and at
 // 26 000 it loses, 29.5 -> 30.0.
-int tokens_per_block(const KvCacheParams& p, bool read, int planes, int elems) {
+}  // namespace
+
+int kv_cache_tokens_per_block(const KvCacheParams& p, bool read, int fmt, int planes) {
+    const int elems = row_chunk(read, fmt);
     const int chunks = p.head_k * (p.plane[0].dim >> 3);  // (of eight elements: kUnroll of them to a thread)
     int tpb = kThreads * kUnroll / chunks;
     const auto groups = [&](int t) { return (p.tokens + t - 1) / t * planes; };
@@ -509,6 +509,8 @@ int tokens_per_block(const KvCacheParams& p, bool read, int planes, int elems) {
     while (tpb > 1 && tpb * chunks > kThreads * elems / 8 && groups(tpb) < 512) tpb >>= 1;
     return tpb < 1 ? 1 : (tpb > kMaxTokens ? kMaxTokens : tpb);
 }
+
+namespace {
 
 template <bool READ, typename Tag, int FMT, int PAIRS>
 hipError_t launch_form(const KvCacheParams& p, int planes, hipStream_t stream) {
@@ -522,8 +524,8 @@ hipError_t launch_form(const KvCacheParams& p, int planes, hipStream_t stream) {
 
 template <bool READ, typename Tag>
 hipError_t launch_tag(KvCacheParams p, int fmt, int pairs, int planes, hipStream_t stream) {
-    const int elems = READ || fmt == 0 ? 8 : 16;  // append_chunk()
-    p.tokens_per_block = tokens_per_block(p, READ, planes, elems);
+    const int elems = row_chunk(READ, fmt);
+    p.tokens_per_block = kv_cache_tokens_per_block(p, READ, fmt, planes);
     for (int i = 0; i < planes; ++i) {
         const uint64_t lanes = (uint64_t)p.plane[i].dim / elems, chunks = lanes * (uint64_t)p.head_k;
         p.plane[i].lanes_magic = (uint32_t)(((1ull << 32) + lanes - 1) / lanes);

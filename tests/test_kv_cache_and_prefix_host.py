@@ -164,3 +164,11 @@ def test_prefix_calls_refuse_more_work_groups_than_a_launch_has():
     assert size(BIG, 8, 2, 8, 4, 128, 128, 0, 0) == 0 and size(64, BIG, 2, 8, 4, 128, 128, 0, 16) == 0
     assert size(64, 8, BIG, 8, 4, 128, 128, 0, 0) == 0 and size(64, 8, 2, 1 << 17, 1, 128, 128, 0, 0) == 0
     assert size(64, 8, 1 << 22, 1, 1, 64, 64, 0, 0) > 0
+
+
+@pytest.mark.parametrize("call", [_append, _read])
+def test_cache_calls_refuse_more_work_groups_than_a_launch_has(call):
+    """A token of 64 heads d 256 is a work-group's share."""
+    lib = _lib.load()
+    assert call(lib, tokens=1 << 24, hk=64, d=256, dv=256) == _lib.DA_ERR_INVALID_ARGUMENT
+    assert b"work-groups" in lib.da_last_error()
