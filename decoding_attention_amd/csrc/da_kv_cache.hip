@@ -350,7 +350,10 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(const KvCacheParams
     const KvPlane& pl = p.plane[blockIdx.y];
     const int64_t tok0 = (int64_t)blockIdx.x * p.tokens_per_block;
     const int lanes = pl.dim / E, chunks = p.head_k * lanes;
-    const int n = (int)min((int64_t)p.tokens_per_block, p.tokens - tok0) * chunks;
+    // (rows behind the last sequence need not be there: they are not read)
+    const int64_t tokens = p.cu_seq ? min(p.tokens, (int64_t)p.cu_seq[p.batch]) : p.tokens;
+    const int n = (int)min((int64_t)p.tokens_per_block, tokens - tok0) * chunks;
+    if (n <= 0) return;
     uint8_t* const pool = reinterpret_cast<uint8_t*>(pl.pool);
     const uint16_t* const src0 = reinterpret_cast<const uint16_t*>(pl.src) + tok0 * pl.src_token;
     bool looked = false;

@@ -389,3 +389,62 @@ def test_attention_over_an_appended_cache(fmt, dtype):
     assert (paged.float() - packed.float()).abs().max().item() <= (2 * move + 5 * u) * big
     if fmt == "16":
         assert torch.equal(k.cpu().view(torch.int16), w.k.view(torch.int16))
+
+
+@pytest.mark.parametrize("fmt", ["16", "fp8", "int8_g64", "int4_tok"])
+@pytest.mark.parametrize("extra", [1, 70, 1 << 22])
+def test_rows_behind_the_last_sequence_need_not_be_there(fmt, extra):
+    """The C call with a count beyond cu_seq[batch] (a captured graph's largest step): k and v hold the sequences' rows alone."""
+    from decoding_attention_amd import _lib
+    lib = _lib.load()
+    c = Cache(fmt, torch.bfloat16, 4, 128, 16, [50, 0, 9], [31, 0, 9], seed=30)
+    dx = {n: x.to(DEV) for n, x in c.x.items()}
+    pk, pv, table, lens, cu = c.gpu_args()
+    pack = 2 if fmt.startswith("int4") else 1
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    forms = {"16": (0, 0), "fp8": (1, 0), "int8_g64": (2, 2), "int4_tok": (3, 1)}[fmt]
+    rc = lib.da_kv_cache_append(dx["k"].data_ptr(), dx["v"].data_ptr(), 512, 128, 512, 128, pk.data_ptr(), pv.data_ptr(),
+                                table.data_ptr(), lens.data_ptr(), cu.data_ptr(), c.tokens + extra, 3, 4, 128, 128, 16,
+                                table.shape[1], c.pages, pk.stride(0) * pack, pv.stride(0) * pack, 1, *forms, ptr(c.dscale["k"]),
+                                ptr(c.dscale["v"]), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, _lib.last_error()
+    torch.cuda.synchronize()
+    c.expected()
+    c.check_pools()
+
+
+def test_replays_of_a_padded_append():
+    """One captured call for steps of up to 96 rows: cu_seq on the device says how many there are, the rows behind hold NaN."""
+    c = Cache("int8_tok", torch.bfloat16, 2, 64, 16, [96, 96], [48, 48], seed=31)
+    pk, pv, table, lens, cu = c.gpu_args()
+    k = torch.full((96, 2, 64), float("nan"), dtype=torch.bfloat16, device=DEV)
+    v = k.clone()
+
+    def step():
+        kv_cache_append(k, v, pk, pv, table, lens, cu, k_scale=c.dscale["k"], v_scale=c.dscale["v"])
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    g = torch.Generator().manual_seed(32)
+    for a, b in ((48, 48), (1, 0), (0, 33), (0, 0), (17, 2)):
+        c.cu = torch.tensor([0, a, a + b], dtype=torch.int32)
+        c.lens, c.tokens = [96 - a, 40 + b], a + b
+        cu.copy_(c.cu), lens.copy_(torch.tensor(c.lens, dtype=torch.int32))
+        for nm, t in (("k", k), ("v", v)):
+            c.x[nm] = torch.randn(a + b, 2, 64, generator=g).to(torch.bfloat16)
+            t.fill_(float("nan"))
+            t[:a + b].copy_(c.x[nm])
+        for nm in c.names:
+            c.pool[nm].copy_(c.dpool[nm].cpu()), c.scale[nm].copy_(c.dscale[nm].cpu())
+        graph.replay()
+        torch.cuda.synchronize()
+        c.at = ora.places(c.table, c.lens, c.cu.tolist(), a + b, c.page, c.pages)
+        if a + b:
+            c.expected()
+        c.check_pools()
