@@ -345,10 +345,8 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
         constexpr uint32_t kOnes = std::is_same<Tag, f16_tag>::value ? 0x3C003C00u : 0x3F803F80u;
         auto exponential = [&](int i) __attribute__((always_inline)) { e[i] = fast_exp2(__builtin_fmaf(s[i], mul, -m)); };
         auto pack = [&](int j) __attribute__((always_inline)) { pw[j] = EL::pack2(e[2 * j], e[2 * j + 1]); };
-        // Exponentials up to kEarly go out beside the score products, the rest beside the first value products; a pair is packed
-        // a slot after its second one.
-        constexpr int kPre = 0, kEarly = 16;
-        auto exps = [](int slot, int slots, int from, int to) { return from + (to - from) * slot / slots; };
+        // The exponentials go out beside the score products, 16 / KS a slot; a pair is packed a slot after its second one.
+        auto exps = [](int slot) { return 16 * slot / KS; };
         auto packs = [&](int from, int to) __attribute__((always_inline)) {  // pairs of exponentials [from, to)
 #pragma unroll
             for (int j = from / 2; j < to / 2; ++j) pack(j);
@@ -362,10 +360,10 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             s_next = MM::mma(kf[ks], q[ks], s_next);
             pin<D>(s_next);
 #pragma unroll
-            for (int i = exps(ks, KS, kPre, kEarly); i < exps(ks + 1, KS, kPre, kEarly); ++i) exponential(i);
+            for (int i = exps(ks); i < exps(ks + 1); ++i) exponential(i);
 #pragma unroll
             for (int i = 4 * CB * ks / KS; i < 4 * CB * (ks + 1) / KS; ++i) read_v(i);
-            packs(ks == 0 ? 0 : exps(ks - 1, KS, kPre, kEarly), exps(ks, KS, kPre, kEarly));
+            packs(ks == 0 ? 0 : exps(ks - 1), exps(ks));
             __builtin_amdgcn_sched_barrier(0);
         });
         wait_lds<2 * CB>();  // V of the first sixteen tokens
@@ -375,17 +373,14 @@ __device__ __forceinline__ void prefix_segment(const PrefixParams& p, uint8_t* c
             const vec8 pf = __builtin_bit_cast(vec8, make_uint4(pw[0], pw[1], pw[2], pw[3]));
             acc[cb] = MM::mma(__builtin_bit_cast(vec8, join(vf[0][cb][0], vf[0][cb][1])), pf, acc[cb]);
             pin<D>(acc[cb]);
-#pragma unroll
-            for (int i = exps(cb, CB, kEarly, 16); i < exps(cb + 1, CB, kEarly, 16); ++i) exponential(i);
             // (the denominator sums the probabilities as the second product sees them)
 #pragma unroll
             for (int j = 4 * cb / CB; j < 4 * (cb + 1) / CB; ++j) l = EL::dot2(pw[j], kOnes, l);
-            packs(cb == 0 ? exps(KS - 1, KS, kPre, kEarly) : exps(cb - 1, CB, kEarly, 16), exps(cb, CB, kEarly, 16));
+            if constexpr (cb == 0) packs(exps(KS - 1), 16);  // (the last slot's: the second value products read them)
 #pragma unroll
             for (int ks = cb; ks < KS / 2; ks += CB) read_k(ks, prev);  // (past the last tile: of whatever lies there, not used)
             __builtin_amdgcn_sched_barrier(0);
         });
-        packs(exps(CB - 1, CB, kEarly, 16), 16);
         wait_lds<KS / 2>();  // V of the other sixteen
         __builtin_amdgcn_sched_barrier(0);
         float mx = -INFINITY;
