@@ -215,11 +215,13 @@ __device__ __forceinline__ float not_finite(uint4 w, float seen) {
 
 // The same for ordinary values at a fourth of the instructions, sixteen integers packed into four words (int4: two).
 // One multiply-add in double precision, x inv + (zero + 1/2 + a constant of 1.5 2^28 or 1.5 2^24), leaves t + 1/2 in the low
-// word as a fixed-point number in units of 2^-24 (int8) or 2^-28 (int4), the integer in its upper bits.  It is off by a unit at
-// most, half from the sum in brackets and half from the result (inv, and the definition's quotient and sum, by less than 2^-40:
-// |zero| < 2^20), and two are added: a fraction of five units and more lies behind the whole number that the definition rounds
-// to, and one that passed the next whole number counts three at most.  The others (of normal values, a lane's sixteen in 200)
-// are settled by the quotient itself.
+// word as a fixed-point number in units of 2^-24 (int8) or 2^-28 (int4), the integer in its upper bits.  It is off from the
+// definition's by less than 1 1/8 units: half from the sum in brackets, half from the result, and from inv and the definition's own
+// quotient 2^-53 of |x / scale| each, less than 2^-32 together and a sixteenth of a unit (|zero| < 2^20, so |x / scale| < 2^20 + 2^9;
+// the definition's sum is below 2^9 and off by 2^-45).  Two units are added, so that the number lies between 7/8 and 3 1/8 units
+// above the definition's: a fraction of five units and more lies behind the whole number that the definition rounds to, and one that
+// passed the next whole number counts three at most.  The others (of normal values, a lane's sixteen in 200) are settled by the
+// quotient itself.
 template <typename Tag, int FMT, int PAIRS>
 __device__ __forceinline__ void quantise(const uint4 (&raw)[2], const uint16_t* src, float factor, int span, uint32_t (&w)[4],
                                          float2& pair) {
