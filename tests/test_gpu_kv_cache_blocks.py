@@ -181,3 +181,10 @@ def test_latent_rows_alone_and_with_values_of_their_own(fmt, tokens):
 @pytest.mark.parametrize("fmt", ora.FORMATS)
 def test_gaps_between_pages_stay_as_they_were(fmt, page):
     run(fmt, 3, 128, 333, page=page, batch=5, seed=page)
+
+
+@pytest.mark.parametrize("fmt", ["16", "int8_tok"])
+@pytest.mark.parametrize("batch", [513, 5000, 70001])
+def test_thousands_of_sequences(fmt, batch):
+    """More sequences than marks, most of them without a row in the call: the second search is many steps long."""
+    run(fmt, 2, 64, 3001, batch=batch, seed=batch)

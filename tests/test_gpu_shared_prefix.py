@@ -605,3 +605,67 @@ def test_an_infinite_value_in_a_sequences_last_token(d, hq, hk, page, lengths):
         o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k, v, cu, most, d, False)
     heads = slice((hk - 1) * (hq // hk), hq)
     check_infinite(o[rows], ref, [(rows.index(b), heads, 5, float("inf")) for b in hit])
+
+
+@pytest.mark.parametrize("page", [0, 16])
+@pytest.mark.parametrize("hq,hk", [(1, 1), (3, 1), (4, 4)])
+def test_a_hundred_thousand_sequences(hq, hk, page):
+    """More sequences than a grid's other axes number, with few rows each; spot checks, and every row is written."""
+    batch, d, prefix = 100_003, 64, 48
+    own = [(b * 7) % 3 for b in range(batch)]
+    g = torch.Generator().manual_seed(hq)
+    q = torch.randn(batch, hq, d, generator=g).half()
+    kp, vp = (torch.randn(prefix, hk, d, generator=g).half() for _ in range(2))
+    cu = torch.tensor([0] + own).cumsum(0)
+    k, v = (torch.randn(int(cu[-1]), hk, d, generator=g).half() for _ in range(2))
+    rows = [0, 1, 2, 1023, 65535, 65536, 99_999, batch - 1]
+    ks, vs = ([t[cu[b]:cu[b + 1]] for b in rows] for t in (k, v))
+    if page:
+        # a page per sequence behind the prefix's three, its first rows the sequence's own
+        pk, pv = (torch.full((3 + batch, page, hk, d), float("nan"), dtype=torch.float16) for _ in range(2))
+        seq = torch.repeat_interleave(torch.arange(batch), torch.tensor(own))
+        at = torch.arange(len(seq)) - cu[seq]
+        for pool, pre, rest in ((pk, kp, k), (pv, vp, v)):
+            pool[:3] = pre.unflatten(0, (3, page))
+            pool[3 + seq, at] = rest
+        ids = torch.arange(3, dtype=torch.int32, device=DEV)
+        table = torch.full((batch, 4), -1, dtype=torch.int32)
+        table[:, 3] = torch.arange(3, 3 + batch)
+        lens = torch.tensor(own, dtype=torch.int32) + prefix
+        o = decoding_attn_paged_shared_prefix_fwd(q.to(DEV), pk.to(DEV), pv.to(DEV), ids, prefix, table.to(DEV), lens.to(DEV), prefix + 2, d, False)
+    else:
+        o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), k.to(DEV), v.to(DEV), cu.to(torch.int32).to(DEV), 2, d, False)
+    assert torch.isfinite(o).all() and (o != 0).any(-1).all()
+    check(o[rows], reference(q[rows], kp, vp, ks, vs, False))
+
+
+@pytest.mark.parametrize("alibi", [False, True])
+def test_a_prefix_past_32_bit_offsets(alibi):
+    """More than 2^32 bytes of packed K: the values are zero but in a few tokens near the ends, whose weights a score of 20
+    raises far above the others' sum."""
+    hk, d, prefix = 32, 128, (1 << 32) // (32 * 128 * 2) + 1000
+    g = torch.Generator().manual_seed(40)
+    q = torch.zeros(3, hk, d)
+    q[:, :, 0] = 1.0
+    q = q.half()
+    kp = torch.zeros(prefix, hk, d, dtype=torch.float16, device=DEV)
+    vp = torch.zeros_like(kp)
+    hot = [5, prefix // 2, prefix - 900, prefix - 1]
+    top = torch.randn(len(hot), hk, generator=g) + 24.0 * d ** 0.5
+    kp[hot, :, 0] = top.half().to(DEV)
+    vals = torch.randn(len(hot), hk, d, generator=g).half()
+    vp[hot] = vals.to(DEV)
+    slopes = torch.full((hk,), 1e-6, device=DEV) if alibi else None
+    empty = kp[:0]
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp, vp, empty, empty, torch.zeros(4, dtype=torch.int32, device=DEV), 0, d, alibi,
+                                        alibi_slopes=slopes)
+    x = top.half().double() / d ** 0.5
+    if alibi:
+        x = x + 1e-6 * (torch.tensor(hot).double() - (prefix - 1))[:, None]
+    rest = torch.full((1, hk), math.log(prefix), dtype=torch.float64)  # all other tokens: score 0, value 0
+    w = torch.softmax(torch.cat([x, rest]), dim=0)[:-1]
+    want = (w[:, :, None] * vals.double()).sum(0)
+    # u = 2^-11: u w |v| for the probabilities, as much for the denominator that sums them, u |o| for the result.  The others are
+    # e^13.2 against e^23.7 and more, a share below 2^-15, which half precision's probabilities may lose whole
+    tol = 2.0 ** -10 * w[:, :, None].mul(vals.double().abs()).sum(0) + (2.0 ** -11 + 2.0 ** -15) * want.abs()
+    assert ((o.cpu().double() - want[None]).abs() <= tol[None]).all()
