@@ -616,11 +616,13 @@ hipError_t launch_form(const PrefixParams& p, int own_wgs, hipStream_t stream) {
 
 template <typename Tag, int D, bool WH>
 hipError_t launch_pages(const PrefixParams& p, int own_wgs, hipStream_t stream) {
-    // how the own part finds a tile's rows: whole tiles in pages of 32 tokens and more (and packed rows), two runs in 16-token
-    // pages, a look-up for every row in smaller ones.  (16-token pages, 64 sequences of 1024 behind 4096, 32/8 heads, two runs
-    // against a look-up per row: d 64 38.4 / 34.4 us, d 128 50.0 / 47.5, d 96 47.1 / 52.3, d 256 98 / 158.)
+    // how the own part finds a tile's rows: whole tiles in pages of 32 tokens and more (and packed rows), a look-up for every row
+    // in smaller ones; at d = 256, whose rows leave no registers for that, two runs in 16-token pages.  (Two runs against a look-up
+    // per row, 64 sequences of 0 .. 1024 behind 4096, 32/8 heads: d 64 33.8 / 31.1 us, d 96 37.3 / 33.7, d 128 49.3 / 47.2, d 256 79
+    // / 126; 128 of 0 .. 256 behind 1024, 32/32 heads: 52 / 46, 82 / 74, 84 / 80, 131 / 247; 16 of 0 .. 512 behind 1024, 32/1 heads:
+    // 10.5 / 10.3, 11.6 / 11.3, 12.8 / 13.0, 17 / 21.)
     if (p.own.block_table == nullptr || p.own.page_shift >= 5) return launch_form<Tag, D, WH, 0>(p, own_wgs, stream);
-    if constexpr (D == 96 || D == 256)
+    if constexpr (D == 256)
         if (p.own.page_shift == 4) return launch_form<Tag, D, WH, 1>(p, own_wgs, stream);
     return launch_form<Tag, D, WH, 2>(p, own_wgs, stream);
 }
