@@ -127,10 +127,11 @@ constexpr size_t gqa_lds_bytes(int nt, int tok_pairs = 0) {
 // PGM: how paged K/V is addressed.  0: one page lookup per tile (pages hold a multiple of 32 tokens; also the packed
 // layout); 1: 16-token pages, a tile is fetched as two runs of 16 tokens, each from one page; 2: smaller pages, every
 // lane looks up the page of the row it loads.
-// CLEAR: V rows past the end become zeros in the tile where the last token, which they repeat, has an infinite value, so that it
-// stays infinite (zero times infinity is no number).  Behind a shared prefix only, where the registers are the prefix's; here they
-// would cost the kernels at d = 256 up to 60 bytes more of scratch a lane.
-template <typename Tag, int D, int DV, int NT, bool PREFETCH, bool WH, int KV8, int PGM, bool CLEAR = false>
+// BEHIND: the segment lies behind a shared prefix, whose part of the kernel sets the registers.  V rows past the end become zeros in
+// the tile where the last token, which they repeat, has an infinite value, so that it stays infinite (zero times infinity is no
+// number; elsewhere this would cost the kernels at d = 256 up to 60 bytes more of scratch a lane).  And the denominator sums the
+// probabilities as rounded for the second product in fp16 as well, as the prefix's does, so that a row's weights add up to one.
+template <typename Tag, int D, int DV, int NT, bool PREFETCH, bool WH, int KV8, int PGM, bool BEHIND = false>
 __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const smem, const int by, const int b,
                                             const int start, const int len, const int c0, const int c1,
                                             const size_t part0, const int part_stride, const bool direct) {
@@ -181,7 +182,8 @@ __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const
     static_assert(!VK || (DV < D && DV % 64 == 0), "value columns inside the key rows");
     static_assert(D % 32 == 0 && DV % 16 == 0 && (kGqaTile * CPR) % 64 == 0, "shape");
     static_assert(!KV8 || (D % 64 == 0 && (kGqaTile * CPRL) % 64 == 0), "8-bit K/V: two k-steps per 16-byte load");
-    static_assert(!CLEAR || (KV8 == 0 && !VK), "16-bit V of its own");
+    constexpr bool kSumPacked = BEHIND && std::is_same<Tag, f16_tag>::value;  // (bf16: rounded one by one, as elsewhere)
+    static_assert(!BEHIND || (KV8 == 0 && !VK), "16-bit V of its own");
     static_assert(!TOK || (!VK && (FMT == kKvInt8 || FMT == kKvInt4)), "per-token factors: integer K/V, V of its own");
 
     const int lane = threadIdx.x & 63;
@@ -424,7 +426,7 @@ __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const
                 *reinterpret_cast<uint4*>(vt + row * VP + ch * 16) = tr.v[i];
             }
         }
-        if constexpr (CLEAR) {
+        if constexpr (BEHIND) {
             if (tok0 + kGqaTile > c1) {
                 // (only where it matters: the tile's last row, one of those past the end, lies in the last register.  Always
                 // cleared, 128 sequences of 0 .. 256 behind 1024, 32/1 heads: d 128 30.0 -> 31.0 us, d 256 41.8 -> 43.1)
@@ -643,7 +645,7 @@ __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const
                         if constexpr (LQ) lq[nt][qg] += tokV[qg][j] != 0.0f ? pq * tokVinv[qg][j] : pe;
                         xg[qg][j] = pq;
                     }
-                } else if constexpr (B4) {
+                } else if constexpr (B4 || kSumPacked) {
                     x[nt][j] = fast_exp2(x[nt][j] - m[nt]);  // (rounded by pack8; the denominator follows below)
                 } else {
                     x[nt][j] = as_second_operand<Tag>(fast_exp2(x[nt][j] - m[nt]));
@@ -654,8 +656,8 @@ __device__ __forceinline__ void gqa_segment(const SweepParams& p, uint8_t* const
             pfg[nt][0] = pf[nt];
 #pragma unroll
             for (int qg = 1; qg < NG; ++qg) pfg[nt][qg] = MM::pack8(xg[qg]);
-            if constexpr (B4 && !TOK) {
-                // the denominator sums the probabilities as rounded for the matrix instruction (it is also what the
+            if constexpr ((B4 && !TOK) || kSumPacked) {
+                // the denominator sums the probabilities as rounded for the matrix instruction (B4: it is also what the
                 // bias is taken out with): a dot product of the packed pairs with ones
                 constexpr uint32_t kOnes = std::is_same<Tag, f16_tag>::value ? 0x3C003C00u : 0x3F803F80u;
                 const uint4 pw = __builtin_bit_cast(uint4, pf[nt]);

@@ -669,3 +669,31 @@ def test_a_prefix_past_32_bit_offsets(alibi):
     # e^13.2 against e^23.7 and more, a share below 2^-15, which half precision's probabilities may lose whole
     tol = 2.0 ** -10 * w[:, :, None].mul(vals.double().abs()).sum(0) + (2.0 ** -11 + 2.0 ** -15) * want.abs()
     assert ((o.cpu().double() - want[None]).abs() <= tol[None]).all()
+
+
+@pytest.mark.parametrize("hq,hk", [(16, 4), (6, 2)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_weights_rounding_is_in_the_denominator_too(dtype, d, hq, hk):
+    """Nearly all the weight on one own token, whose unnormalised probability, some 2^7 of the running maximum's, is rounded
+    where a step is largest (1.0 to 1.1 times a power of two): rounded in the sum over V alone it would scale the row by up to half a
+    step, beside the result's own, and the values are such that this is a whole one.  (The token lies in the last tile of 129 tokens, so
+    that it follows the first tile's maximum in the same wave, also where four waves take tiles in turn, and the batch is large enough
+    for sequences that are not split.)"""
+    batch, rows = 300, list(range(0, 300, 9))
+    g = torch.Generator().manual_seed(d + hq)
+    low = -20.0 * d ** 0.5
+    q = torch.zeros(batch, hq, d)
+    q[:, :, 0] = 1.0
+    k = torch.zeros(batch, 129, hk, d)
+    k[:, :, :, 0] = low
+    k[:, 0, :, 0] = 0.0
+    k[:, 128, :, 0] = (7.0 + 0.13 * torch.rand(batch, hk, generator=g)) * math.log(2.0) * d ** 0.5
+    v = 1.0 + 0.1 * torch.rand(batch, 129, hk, d, generator=g)
+    kp, vp = torch.zeros(1, hk, d), torch.ones(1, hk, d)
+    kp[:, :, 0] = low
+    q, k, v, kp, vp = (t.to(dtype) for t in (q, k, v, kp, vp))
+    ks, vs = list(k), list(v)
+    kk, vv, cu, most = packed(ks, vs, hk, d, dtype)
+    o = decoding_attn_shared_prefix_fwd(q.to(DEV), kp.to(DEV), vp.to(DEV), kk, vv, cu, most, d, False)
+    check(o[rows], some(q, kp, vp, ks, vs, False, rows))
