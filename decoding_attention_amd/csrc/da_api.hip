@@ -1429,8 +1429,8 @@ PrefixPlan make_prefix_plan(size_t prefix_len, size_t own_max, size_t own_total,
     // d 64 0.48 and 0.75; d 256 0.85 alone) or beside a second one; while both run the own ones lose a fifth.  Up to d = 128 a
     // CU holds one of each kind, or two; at d = 256 one.  The row tiles of a (KV head, split) pair are kept on one XCD unless
     // dealing them out over all eight is faster with the K/V read into every L2 (64/2 heads d 128, 82 sequences behind 5120
-    // tokens: 21 row tiles a pair, 48 -> 38 us).  Against ten forced counts on 36 shapes the choice is within 6 % of the best in 31 and up
-    // to 17 % behind in five (256 sequences of 0 .. 128 behind 16384, d 64: 69 us against 59 with eight splits).
+    // tokens: 21 row tiles a pair, 48 -> 38 us).  Against ten forced counts on 36 shapes the choice is within 6 % of the best in 30 and up
+    // to 22 % behind in six (256 sequences of 0 .. 128 behind 16384, d 64: 73 us against 60 with eight splits).
     pl.row_tiles = (int)((rows + da::kPrefixRows - 1) / da::kPrefixRows);
     const double own_us = own_max > 0 ? 4.0 * (double)own_total * (double)head_k * (double)dim / 5.0e6 + 6.0 : 0.0;
     const double kv_us = 4.0 * (double)prefix_len * (double)head_k * (double)dim / 5.0e6;

@@ -13,8 +13,8 @@
 // stored.
 //
 // What bounds them: a read moves 5 to 6 TB/s, as much as a copy (24 sequences of 0 .. 1300 tokens, 16-bit, 4 heads d 256: 131 MB in
-// 23 to 27 us; 114 000 int4 tokens of 8 heads d 128 with a pair per 64: 615 MB in 116 to 131).  An append spends 12 vector
-// instructions an element on exact quotients and runs at 4.5 TB/s (26 000 tokens of 8 heads d 128, int8 per 64: 168 MB in 37 to 38 us).
+// 22 to 27 us; 114 000 int4 tokens of 8 heads d 128 with a pair per 64: 615 MB in 116 to 133).  An append spends 12 vector
+// instructions an element on exact quotients and runs at 4.4 TB/s (26 000 tokens of 8 heads d 128, int8 per 64: 168 MB in 37 to 40 us).
 // Small calls are the launch and the three trips of the look-up: 3 to 4 us, for one sequence or 64.
 #include "da_kv_cache.h"
 

@@ -23,9 +23,9 @@
 // that a row's weights still add up to one.
 //
 // What bounds it: the prefix part alone is power-limited matrix work, 256 sequences behind 16384 tokens, 32/8 heads d 128:
-// 73 us, 940 TFLOP/s with two work-groups per CU; with one per CU it is the latency of a tile's chain (0.6 us for 0.25 us of
-// products).  With own tokens (542 MB, alone 95 us) the launch takes 136 us at least and 146 to 168 in the median of runs on several
-// GPUs, where one part after the other takes 168.  128 rows a work-group: with 64 the K/V reads from LDS per product double, with
+// 71 to 73 us, 960 TFLOP/s with two work-groups per CU; with one per CU it is the latency of a tile's chain (0.6 us for 0.25 us of
+// products).  With own tokens (542 MB, alone 95 us) the launch takes 135 us at least and 144 to 168 in the median of runs on several
+// GPUs, where one part after the other takes 166.  128 rows a work-group: with 64 the K/V reads from LDS per product double, with
 // 256 the splits, and so the partials, do.  Wide rows (d 256) leave one work-group per CU and its chain: 1056 rows behind 32768
 // tokens 66 us, 540 TFLOP/s; there the partials of a short call (8192 tokens: 18 MB out and back) are more than twice the K/V.
 #pragma once

@@ -2,7 +2,7 @@
 // j to thread j mod G), each adds up its share with a running maximum, and the G sums meet in LDS in thread order, so the result
 // does not depend on timing.  One thread per (row, four columns, share).
 //
-// Bound by the trips to memory that a thread makes one after the other, 4.5 us for the smallest call (the length, the partials'
+// Bound by the trips to memory that a thread makes one after the other, 3 to 4 us for the smallest call (the length, the partials'
 // places, the partials); large ones read at 3 TB/s what the sweep has just written past the L2 (8192 rows of d 128, five partials
 // each, 21 MB: 7 us; 1056 rows of d 256 and 17 partials, 18 MB: 5.8).  With G = 1 and 20 partials of 2048 rows (17 MB, d 128) the
 // merge took 9.3 us, half of its sweep's time.
